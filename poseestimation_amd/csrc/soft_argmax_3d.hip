@@ -454,7 +454,7 @@ __global__ __launch_bounds__(kShareThreads, 4) void soft_argmax_3d_resident(
 #pragma unroll
         for (int k = 0; k < NV4; ++k) {
             const unsigned i = first + (k * kShareThreads + tid) * 4;
-            const vec4f d = (v[k] - mref) * 1.44269504088896340736f;  // exp_neg, with the packed subtract and multiply
+            const vec4f d = (v[k] - mref) * 1.44269504088896340736f;  // exp_neg, four at a time
             vec4f e;
 #pragma unroll
             for (int l = 0; l < 4; ++l) e[l] = __builtin_amdgcn_exp2f(d[l]);
