@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define MVX_VERSION 200 /* major*10000 + minor*100 + patch; 0.2.0 adds the backward entry points */
+#define MVX_VERSION 300 /* major*10000 + minor*100 + patch; 0.2.0 adds the backward entry points, 0.3.0 the sequence operators */
 
 enum mvx_status {
     MVX_OK = 0,
@@ -348,6 +348,116 @@ int mvx_unity_points(const float* points, const int32_t* joint_order, int64_t n_
  */
 int mvx_realtime_tail(float* ring, const float* new_pose, int ring_pos, int n_steps, int n_joints, const double* hat,
                       int window, const int32_t* joint_order, float scale, int filtered, float* out, void* stream);
+
+/* ---- Operators over sequences of frames --------------------------------------------------------------------------------
+ * What a model over the tokens of a sequence needs next to the filter and the pose ring above: layer norm, rotary positions
+ * with several axes, attention with a sliding window, and its form for one new token of a stream.  They have no counterpart
+ * in the reference.  `dtype` is an mvx_dtype; tensors of that type are float32, bfloat16 or float16; arithmetic, softmax
+ * statistics and sums are float32, results are rounded once.  Tokens are [n_seqs][n_tokens][heads][dim].
+ */
+enum mvx_dtype { MVX_F32 = 0, MVX_BF16 = 1, MVX_F16 = 2 };
+
+/*
+ * Layer norm of each of `rows` rows of `width` values: y = (x - mean) / sqrt(var + eps) * weight + bias.
+ * x, y          [rows][width] of dtype
+ * weight, bias  [width], float32 if param_f32 != 0, else dtype; NULL = 1 and 0
+ * stats         [rows][2] float32 out: mean and 1 / sqrt(var + eps), what the backward reads; or NULL
+ */
+int mvx_layer_norm(const void* x, const void* weight, const void* bias, int dtype, int param_f32, int64_t rows, int64_t width,
+                   float eps, void* y, float* stats, void* stream);
+
+/*
+ * Backward of mvx_layer_norm.  With h = (x - mean) r, a = grad_y * weight: grad_x = r (a - mean(a) - h mean(a h)),
+ * grad_weight = sum over rows of grad_y h, grad_bias = sum over rows of grad_y (summed in a fixed order, no atomics).
+ * stats                    what the forward call wrote
+ * grad_x                   [rows][width] of dtype, or NULL
+ * grad_weight, grad_bias   [width] of the parameters' type, or NULL
+ * workspace                mvx_layer_norm_backward_workspace_bytes() bytes, 4-byte aligned (not needed when grad_weight and
+ *                          grad_bias are NULL)
+ */
+size_t mvx_layer_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t width);
+int mvx_layer_norm_backward(const void* grad_y, const void* x, const void* weight, const float* stats, int dtype, int param_f32,
+                            int64_t rows, int64_t width, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions with several axes: turns the first 2 * sum(sections) values of every head of q and k (k_heads = 0: q
+ * alone) pair by pair.  Pair i lies in the section of one axis and turns by position[axis] * base^-e, e = the pair's place in
+ * its section / the section's pairs (shared_spectrum == 0) or i / all pairs (shared_spectrum != 0); pairs are (i, i + pairs)
+ * or, with adjacent_pairs != 0, (2i, 2i + 1); values behind the pairs are copied.  Angles are float64.  inverse != 0 turns the
+ * other way: the backward of the call with inverse == 0.
+ * q, k         [n_seqs][n_tokens][heads][dim] of dtype with strides {sequence, token, head} in elements (HOST arrays of 3),
+ *              the last axis contiguous
+ * positions    [n_seqs][n_tokens][n_axes] of position_type (0 int32, 1 int64, 2 float32, 3 float64), position_seq_stride
+ *              elements from one sequence to the next (0: all share one)
+ * sections     HOST array of n_axes (1 to 4) pair counts, at most 128 pairs in all
+ * q_out, k_out contiguous; must not overlap the inputs
+ */
+int mvx_rotate_positions(const void* q, const int64_t* q_strides, int q_heads, const void* k, const int64_t* k_strides,
+                         int k_heads, int dtype, int64_t n_seqs, int64_t n_tokens, int dim, const void* positions,
+                         int position_type, int64_t position_seq_stride, int n_axes, const int32_t* sections, double base,
+                         int shared_spectrum, int adjacent_pairs, int inverse, void* q_out, void* k_out, void* stream);
+
+/*
+ * Attention with a sliding window and first tokens that stay visible.  Query i of a sequence sees key j iff j <= i + right and
+ * (j >= i - left or j < sinks), j < lengths[sequence] and visible[sequence][j]; out_i = softmax over the seen keys of
+ * scale q_i . k_j, times v_j.  A query that sees no key, and a query at or behind its sequence's length, gives zeros.  Values
+ * of hidden tokens (not visible, or behind the length) never enter a product, whatever they hold.
+ * q            [n_seqs][n_tokens][heads][dim] of dtype; k, v [n_seqs][n_tokens][kv_heads][dim] (head h reads key/value head
+ *              h / (heads / kv_heads)); strides {sequence, token, head} in elements (HOST arrays of 3), the last axis
+ *              contiguous, base and strides multiples of 16 bytes; dim a multiple of 8, at most 128
+ * left, right  >= 0; values beyond n_tokens mean no limit
+ * lengths      [n_seqs] int64 or NULL (values outside 0 .. n_tokens are clamped);  visible [n_seqs][n_tokens] bytes or NULL
+ * out          [n_seqs][n_tokens][heads][dim], contiguous
+ * lse          [n_seqs][heads][n_tokens] float32 out: log2 of the softmax denominator, what the backward reads; or NULL
+ */
+int mvx_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
+                         int64_t left, int64_t right, int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
+                         void* out, float* lse, void* stream);
+
+/*
+ * Backward of mvx_window_attention: gradients of q, k and v given grad_out.  Summed in a fixed order, no atomics; tokens at or
+ * behind a sequence's length, and keys that are hidden, get zeros.
+ * out, lse        what the forward call wrote
+ * grad_out        as q: [n_seqs][n_tokens][heads][dim] with strides
+ * grad_q          [n_seqs][n_tokens][heads][dim]; grad_k, grad_v [n_seqs][n_tokens][kv_heads][dim]; contiguous
+ * workspace       mvx_window_attention_backward_workspace_bytes() bytes, 16-byte aligned
+ */
+size_t mvx_window_attention_backward_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
+                                                     int64_t left, int64_t sinks);
+int mvx_window_attention_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                  const void* v, const int64_t* v_strides, const void* out, const float* lse,
+                                  const void* grad_out, const int64_t* grad_strides, int dtype, int64_t n_seqs,
+                                  int64_t n_tokens, int heads, int kv_heads, int dim, int64_t left, int64_t right,
+                                  int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible, void* grad_q,
+                                  void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One new token per stream over a ring of cached tokens: mvx_window_attention's row of that token for left = window - 1,
+ * right = 0.  A stream keeps sinks + window slots; token t (counted from 0) lies in slot t for t < sinks, else in slot
+ * sinks + (t - sinks) % window.  The call stores k and v in the slot of token lengths[stream], attends over the slots held,
+ * and adds 1 to lengths[stream], all on the device.  A negative length marks an idle stream: its cache and length stay as
+ * they are and its row of out is zero.
+ * q            [n_seqs][heads][dim] of dtype; k, v [n_seqs][kv_heads][dim]; contiguous
+ * k_cache, v_cache  [n_seqs][sinks + window][kv_heads][dim], read and written;  lengths [n_seqs], read and written
+ * out          [n_seqs][heads][dim]
+ * workspace    mvx_window_attention_step_workspace_bytes() bytes, 4-byte aligned; q, caches: 16-byte aligned
+ */
+size_t mvx_window_attention_step_workspace_bytes(int64_t n_seqs, int heads, int kv_heads, int dim, int64_t window, int64_t sinks);
+int mvx_window_attention_step(const void* q, const void* k, const void* v, int dtype, int64_t n_seqs, int heads, int kv_heads,
+                              int dim, int64_t window, int64_t sinks, float scale, void* k_cache, void* v_cache,
+                              int64_t* lengths, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Fills the ring of mvx_window_attention_step from the first lengths[sequence] tokens of recorded sequences: the first `sinks`
+ * and the last `window` of them go to their slots, other slots stay as they are (lengths <= 0: none; above n_tokens: taken as
+ * n_tokens).  lengths is then what the next step takes.
+ * k, v  [n_seqs][n_tokens][kv_heads][dim] as for mvx_window_attention;  caches as for mvx_window_attention_step
+ */
+int mvx_window_cache_fill(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
+                          const int64_t* lengths, int64_t n_seqs, int64_t n_tokens, int kv_heads, int dim, int64_t window,
+                          int64_t sinks, void* k_cache, void* v_cache, void* stream);
 
 /*
  * HOST function (no device work): fills view_pairs with the sorted pairs that n_draws successive calls of

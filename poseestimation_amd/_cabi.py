@@ -13,6 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmvx.so")
 
 MVX_OK, MVX_ERR_INVALID_ARGUMENT, MVX_ERR_HIP, MVX_ERR_WORKSPACE, MVX_ERR_UNSUPPORTED = range(5)
+F32, BF16, F16 = range(3)  # mvx_dtype
 AGG_SUM, AGG_CONF, AGG_MAX, AGG_SOFTMAX = range(4)
 SELECT_NO_UNPROJECT_BRICKS = 1
 SELECT_NO_DLT_ROWS = 2
@@ -58,6 +59,20 @@ SIGNATURES = {
     "mvx_draw_view_pairs": (_int, [_vp, _vp, _int, _i64, _vp]),
     "mvx_savgol_filter": (_int, [_vp, _i64, _i64, _vp, _int, _vp, _vp]),
     "mvx_unity_points": (_int, [_vp, _vp, _i64, _int, _f32, _vp, _vp]),
+    "mvx_layer_norm": (_int, [_vp, _vp, _vp, _int, _int, _i64, _i64, _f32, _vp, _vp, _vp]),
+    "mvx_layer_norm_backward_workspace_bytes": (_sz, [_int, _i64, _i64]),
+    "mvx_layer_norm_backward": (_int, [_vp, _vp, _vp, _vp, _int, _int, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mvx_rotate_positions": (_int, [_vp, _vp, _int, _vp, _vp, _int, _int, _i64, _i64, _int, _vp, _int, _i64, _int, _vp,
+                                    ctypes.c_double, _int, _int, _int, _vp, _vp, _vp]),
+    "mvx_window_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _f32,
+                                    _vp, _vp, _vp, _vp, _vp]),
+    "mvx_window_attention_backward_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int, _i64, _i64]),
+    "mvx_window_attention_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _int, _int,
+                                             _int, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mvx_window_attention_step_workspace_bytes": (_sz, [_i64, _int, _int, _int, _i64, _i64]),
+    "mvx_window_attention_step": (_int, [_vp, _vp, _vp, _int, _i64, _int, _int, _int, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp,
+                                         _sz, _vp]),
+    "mvx_window_cache_fill": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _int, _int, _i64, _i64, _vp, _vp, _vp]),
     "mvx_realtime_tail": (_int, [_vp, _vp, _int, _int, _int, _vp, _int, _vp, _f32, _int, _vp, _vp]),
 }
 

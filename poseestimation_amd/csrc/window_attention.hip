@@ -1,0 +1,234 @@
+// Attention with a sliding window and first tokens that stay visible, forward.
+//
+//   key j is seen by query i iff j <= i + right and (j >= i - left or j < sinks), j < length, visible[j]
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i) over the seen keys; a row that sees none is zero
+//
+// One workgroup of 4 waves takes 128 queries of one head, 32 per wave, and walks the tiles of 64 keys that any of them
+// sees: first those of the sinks, then the window.  Scores come out transposed (keys in registers, queries in lanes), so the
+// softmax of a query runs inside a lane and its partner 32 lanes on, with a running maximum and sum, and the weighted sum of
+// the values takes the scores where they lie.  A tile is held in LDS for all four waves and the next one travels from memory
+// meanwhile; tiles that every query sees whole skip the mask, and a wave skips a tile that none of its queries sees.
+// Scores and sums are float32; the weights (at most 1) are rounded to the element type for the second product, the sum that
+// divides the result is taken before that rounding.
+#include "attention_tiles.h"
+
+namespace mvx {
+
+namespace {
+
+constexpr int kWaves = 4, kBQ = 32 * kWaves, kBK = 64;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kWaves) void window_attention(TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a,
+                                                                int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
+    using Tl = Tiles<T, DP>;
+    __shared__ __attribute__((aligned(16))) T k_tile[kBK * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T v_tile[kBK * Tl::LD];
+    // heads that share keys, then blocks of queries, are neighbours on one XCD
+    unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int share = a.heads / a.kv_heads;
+    const int in_group = id % share;
+    id /= share;
+    const int block = id % q_blocks;
+    id /= q_blocks;
+    const int kv_head = id % a.kv_heads;
+    const int64_t seq = id / a.kv_heads;
+    const int head = kv_head * share + in_group;
+    const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
+    const int length = seq_length(a, seq);
+    const int q0 = block * kBQ, mine = q0 + wave * 32 + (lane_id() & 31);
+
+    const T* kb = static_cast<const T*>(k.p) + seq * k.seq + kv_head * k.head;
+    const T* vb = static_cast<const T*>(v.p) + seq * v.seq + kv_head * v.head;
+    typename Tl::Frag qf;
+    Tl::load_column(qf, static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head, a.dim,
+                    mine < length);
+
+    // the keys this lane's query sees: j <= hi and (j >= lo or j < sinks)
+    const int hi = mine < length ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
+    int tiles = 0, sink_tiles = 0, first_tile = 0;
+    if (q0 < length) {
+        first_tile = max(0, q0 - a.left) / kBK;
+        tiles = min(q0 + kBQ - 1 + a.right, length - 1) / kBK + 1 - first_tile;
+        sink_tiles = min((min(a.sinks, length) + kBK - 1) / kBK, first_tile);
+        tiles += sink_tiles;
+    }
+    const int w0 = q0 + wave * 32;  // the wave's first query
+
+    v16f acc[DP / 32];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
+    float top = -kInf, sum = 0.0f;
+
+    TileInFlight<T, DP, kBK, 64 * kWaves> k_next, v_next;
+    if (tiles > 0) {
+        const int k0 = (sink_tiles > 0 ? 0 : first_tile) * kBK;
+        k_next.load(kb, k.token, k0, length, a.dim);
+        v_next.load(vb, v.token, k0, length, a.dim);
+    }
+    for (int t = 0; t < tiles; ++t) {
+        const int k0 = (t < sink_tiles ? t : first_tile + t - sink_tiles) * kBK;
+        const uint64_t keep = tokens_kept(a, seq, k0, length);
+        __syncthreads();  // the previous tile is read
+        k_next.store(k_tile, keep);
+        v_next.store(v_tile, keep);
+        __syncthreads();
+        if (t + 1 < tiles) {
+            const int n0 = (t + 1 < sink_tiles ? t + 1 : first_tile + t + 1 - sink_tiles) * kBK;
+            k_next.load(kb, k.token, n0, length, a.dim);
+            v_next.load(vb, v.token, n0, length, a.dim);
+        }
+        if (w0 >= length || k0 > min(w0 + 31 + a.right, length - 1) || (k0 + kBK <= w0 - a.left && k0 >= a.sinks)) continue;
+        v16f s[kBK / 32];
+#pragma unroll
+        for (int b = 0; b < kBK / 32; ++b) s[b] = Tl::rows_times(k_tile + 32 * b * Tl::LD, qf, v16f{});
+        const bool whole = keep == ~0ull && w0 + 31 < length && k0 + kBK - 1 <= w0 + a.right && (k0 >= w0 + 31 - a.left || k0 + kBK <= a.sinks);
+        float most = -kInf;
+        if (whole) {
+#pragma unroll
+            for (int b = 0; b < kBK / 32; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[b][i] *= a.scale_log2;
+                    most = fmaxf(most, s[b][i]);
+                }
+        } else {
+            const int at = k0 + 4 * half;  // register i of block b is key at + 32 b + 8 (i / 4) + i % 4
+            const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
+            const uint64_t bits = keep >> (4 * half);
+#pragma unroll
+            for (int b = 0; b < kBK / 32; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 32 * b + 8 * (i / 4) + i % 4;
+                    const bool seen = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1);
+                    s[b][i] = seen ? s[b][i] * a.scale_log2 : -kInf;
+                    most = fmaxf(most, s[b][i]);
+                }
+        }
+        most = fmaxf(both_halves_max(most), top);
+        const float ref = most == -kInf ? 0.0f : most;
+        if (__any(most > top)) {
+            const float f = __builtin_amdgcn_exp2f(top - ref);  // top = -inf: 0
+            sum *= f;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= f;
+            top = most;
+        }
+#pragma unroll
+        for (int b = 0; b < kBK / 32; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(s[b][i] - ref);
+                sum += s[b][i];
+            }
+            Tl::cols_times(v_tile + 32 * b * Tl::LD, s[b], acc);
+        }
+    }
+    sum = both_halves_sum(sum);
+    if (__any(mine < length && !(all_finite(acc) && sum < kInf))) {
+        const T* qr = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head;
+        top = -kInf;
+        sum = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
+        for_seen_keys(a, seq, lo, hi, [&](int j) { top = fmaxf(top, dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2); });
+        // every score a NaN: a reference of 0 keeps the row apart from one that sees nothing
+        if (hi >= 0) for_seen_keys(a, seq, lo, hi, [&](int) { top = fmaxf(top, -3.0e38f); });
+        for_seen_keys(a, seq, lo, hi, [&](int j) {
+            const float p = __builtin_amdgcn_exp2f(dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2 - top);
+            sum += p;
+            add_row<T, DP>(acc, p, vb + j * v.token, a.dim);
+        });
+    }
+    if (mine >= a.n_tokens) return;
+    const bool none = top == -kInf;
+    const float inv = none ? 0.0f : 1.0f / sum;
+    if (lse != nullptr && half == 0)
+        lse[(seq * a.heads + head) * a.n_tokens + mine] = none ? 0.0f : top + __builtin_amdgcn_logf(sum);  // log2
+    T* o = out + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = 32 * dt + 8 * b + 4 * half;
+            if (d >= a.dim) continue;
+            vec4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(none ? 0.0f : acc[dt][4 * b + e] * inv);
+            *reinterpret_cast<vec4*>(o + d) = w;
+        }
+}
+
+}  // namespace
+
+// Checks that the forward and the backward share; fills `s`.
+int attention_shape(const char* name, int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
+                    int64_t left, int64_t right, int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
+                    AttentionShape* s) {
+    MVX_REQUIRE(dtype == MVX_F32 || dtype == MVX_BF16 || dtype == MVX_F16, MVX_ERR_INVALID_ARGUMENT, "%s: unknown element type %d",
+                name, dtype);
+    MVX_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0, MVX_ERR_INVALID_ARGUMENT,
+                "%s: bad shape n_seqs=%lld n_tokens=%lld heads=%d kv_heads=%d", name, (long long)n_seqs, (long long)n_tokens,
+                heads, kv_heads);
+    MVX_REQUIRE(dim > 0 && dim % 8 == 0, MVX_ERR_INVALID_ARGUMENT, "%s: head dimension %d is not a multiple of 8", name, dim);
+    MVX_REQUIRE(dim <= 128, MVX_ERR_UNSUPPORTED, "%s: head dimension %d above 128", name, dim);
+    MVX_REQUIRE(n_tokens <= (1 << 30), MVX_ERR_UNSUPPORTED, "%s: more than 2^30 tokens", name);
+    MVX_REQUIRE(left >= 0 && right >= 0 && sinks >= 0, MVX_ERR_INVALID_ARGUMENT, "%s: bad window (%lld, %lld) or sinks %lld", name,
+                (long long)left, (long long)right, (long long)sinks);
+    MVX_REQUIRE(scale > 0.0f && scale < kInf, MVX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", name);
+    const auto within = [&](int64_t x) { return static_cast<int>(x < n_tokens ? x : n_tokens); };
+    *s = {n_seqs, static_cast<int>(n_tokens), heads, kv_heads, dim, within(left), within(right), within(sinks), scale * kLog2e,
+          lengths, visible};
+    return MVX_OK;
+}
+
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, TokenTensor* t) {
+    MVX_REQUIRE(p != nullptr && strides != nullptr, MVX_ERR_INVALID_ARGUMENT, "%s: null pointer (%s)", name, what);
+    const int64_t vec = 16 / element_bytes(dtype);
+    MVX_REQUIRE(aligned16(p) && strides[0] % vec == 0 && strides[1] % vec == 0 && strides[2] % vec == 0, MVX_ERR_INVALID_ARGUMENT,
+                "%s: %s must be 16-byte aligned in its base and strides", name, what);
+    *t = {p, strides[0], strides[1], strides[2]};
+    return MVX_OK;
+}
+
+}  // namespace mvx
+
+extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                    const void* v, const int64_t* v_strides, int dtype, int64_t n_seqs, int64_t n_tokens,
+                                    int heads, int kv_heads, int dim, int64_t left, int64_t right, int64_t sinks, float scale,
+                                    const int64_t* lengths, const uint8_t* visible, void* out, float* lse, void* stream) {
+    using namespace mvx;
+    const char* name = "mvx_window_attention";
+    AttentionShape s;
+    int rc = attention_shape(name, dtype, n_seqs, n_tokens, heads, kv_heads, dim, left, right, sinks, scale, lengths, visible, &s);
+    if (rc != MVX_OK) return rc;
+    if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
+    TokenTensor qt, kt, vt;
+    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, &qt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, &vt)) != MVX_OK) return rc;
+    MVX_REQUIRE(out != nullptr && aligned16(out), MVX_ERR_INVALID_ARGUMENT, "%s: out is null or not 16-byte aligned", name);
+    const int q_blocks = static_cast<int>((n_tokens + kBQ - 1) / kBQ);
+    MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
+                name);
+    const unsigned blocks = static_cast<unsigned>(n_seqs * heads * q_blocks);
+    return with_element(dtype, name, [&](auto zero) -> int {
+        using T = decltype(zero);
+        const auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
+                               static_cast<T*>(out), lse);
+        };
+        if (dim <= 32)
+            launch(window_attention<T, 32>);
+        else if (dim <= 64)
+            launch(window_attention<T, 64>);
+        else if (dim <= 96)
+            launch(window_attention<T, 96>);
+        else
+            launch(window_attention<T, 128>);
+        MVX_CHECK_LAUNCH(name);
+        return MVX_OK;
+    });
+}

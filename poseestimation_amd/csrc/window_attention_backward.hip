@@ -1,0 +1,381 @@
+// Backward of the windowed attention.  With p_ij = exp(scale q_i . k_j - lse_i) over the seen pairs and g = dL/do:
+//
+//   dv_j = sum_i p_ij g_i          dp_ij = g_i . v_j         delta_i = g_i . o_i = sum_j p_ij dp_ij
+//   ds_ij = p_ij (dp_ij - delta_i)  dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i
+//
+// Two kernels, each recomputing p from the scores and the forward's lse, so that every gradient is summed in registers in a
+// fixed order and no atomics are needed (two more products of five; the result is the same in every run):
+//   1. queries in lanes, walking the tiles of keys as the forward does: delta and dq;
+//   2. keys in lanes, walking the tiles of queries that see them, over all heads that share the keys: dk and dv.
+// In the second a block of sink keys is seen by the whole rest of the sequence.  The queries beyond the block's own window
+// are therefore cut into chunks that run as workgroups of their own and leave partial sums in float32; the block itself runs
+// in a later launch and adds them in order.
+// p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.
+#include "attention_tiles.h"
+
+namespace mvx {
+
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlock = 32 * kWaves, kTile = 64;
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float factor, T* row, int dim) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const int half = lane_id() >> 5;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = 32 * dt + 8 * b + 4 * half;
+            if (d >= dim) continue;
+            vec4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[dt][4 * b + e] * factor);
+            *reinterpret_cast<vec4*>(row + d) = w;
+        }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
+                                                                TokenTensor g, AttentionShape a, float scale, int q_blocks,
+                                                                const float* __restrict__ lse, float* __restrict__ delta,
+                                                                T* __restrict__ dq) {
+    using Tl = Tiles<T, DP>;
+    __shared__ __attribute__((aligned(16))) T k_tile[kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T v_tile[kTile * Tl::LD];
+    unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int share = a.heads / a.kv_heads;
+    const int in_group = id % share;
+    id /= share;
+    const int block = id % q_blocks;
+    id /= q_blocks;
+    const int kv_head = id % a.kv_heads;
+    const int64_t seq = id / a.kv_heads;
+    const int head = kv_head * share + in_group;
+    const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
+    const int length = seq_length(a, seq);
+    const int q0 = block * kBlock, w0 = q0 + wave * 32, mine = w0 + (lane_id() & 31);
+
+    const T* kb = static_cast<const T*>(k.p) + seq * k.seq + kv_head * k.head;
+    const T* vb = static_cast<const T*>(v.p) + seq * v.seq + kv_head * v.head;
+    const bool live = mine < length;
+    typename Tl::Frag qf, gf;
+    Tl::load_column(qf, static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head, a.dim, live);
+    Tl::load_column(gf, static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head, a.dim, live);
+    float my_delta, my_lse = 0.0f;
+    {
+        typename Tl::Frag of;
+        Tl::load_column(of, static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head, a.dim,
+                        live);
+        my_delta = both_halves_sum(Tl::dot(gf, of));
+    }
+    const int64_t at_row = (seq * a.heads + head) * a.n_tokens + mine;
+    if (live) my_lse = lse[at_row];
+    if (mine < a.n_tokens && half == 0) delta[at_row] = my_delta;
+
+    const int hi = live ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
+    int tiles = 0, sink_tiles = 0, first_tile = 0;
+    if (q0 < length) {
+        first_tile = max(0, q0 - a.left) / kTile;
+        tiles = min(q0 + kBlock - 1 + a.right, length - 1) / kTile + 1 - first_tile;
+        sink_tiles = min((min(a.sinks, length) + kTile - 1) / kTile, first_tile);
+        tiles += sink_tiles;
+    }
+    v16f acc[DP / 32];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
+
+    TileInFlight<T, DP, kTile, kThreads> k_next, v_next;
+    if (tiles > 0) {
+        const int k0 = (sink_tiles > 0 ? 0 : first_tile) * kTile;
+        k_next.load(kb, k.token, k0, length, a.dim);
+        v_next.load(vb, v.token, k0, length, a.dim);
+    }
+    for (int t = 0; t < tiles; ++t) {
+        const int k0 = (t < sink_tiles ? t : first_tile + t - sink_tiles) * kTile;
+        const uint64_t keep = tokens_kept(a, seq, k0, length);
+        __syncthreads();
+        k_next.store(k_tile, keep);
+        v_next.store(v_tile, keep);
+        __syncthreads();
+        if (t + 1 < tiles) {
+            const int n0 = (t + 1 < sink_tiles ? t + 1 : first_tile + t + 1 - sink_tiles) * kTile;
+            k_next.load(kb, k.token, n0, length, a.dim);
+            v_next.load(vb, v.token, n0, length, a.dim);
+        }
+        if (w0 >= length || k0 > min(w0 + 31 + a.right, length - 1) || (k0 + kTile <= w0 - a.left && k0 >= a.sinks)) continue;
+        const bool whole = keep == ~0ull && w0 + 31 < length && k0 + kTile - 1 <= w0 + a.right &&
+                           (k0 >= w0 + 31 - a.left || k0 + kTile <= a.sinks);
+        const int at = k0 + 4 * half;
+        const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
+        const uint64_t bits = keep >> (4 * half);
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b) {
+            v16f s = Tl::rows_times(k_tile + 32 * b * Tl::LD, qf, v16f{});
+            const v16f dp = Tl::rows_times(v_tile + 32 * b * Tl::LD, gf, v16f{});
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float ds = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -my_lse)) * (dp[i] - my_delta);
+                if (whole) {
+                    s[i] = ds;
+                } else {
+                    const int r = 32 * b + 8 * (i / 4) + i % 4;
+                    s[i] = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1) ? ds : 0.0f;
+                }
+            }
+            Tl::cols_times(k_tile + 32 * b * Tl::LD, s, acc);
+        }
+    }
+    if (__any(live && !all_finite(acc))) {
+        const T* qr = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head;
+        const T* gr = static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
+        for_seen_keys(a, seq, lo, hi, [&](int j) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, kb + j * k.token, a.dim), a.scale_log2, -my_lse));
+            add_row<T, DP>(acc, p * (dot_rows(gr, vb + j * v.token, a.dim) - my_delta), kb + j * k.token, a.dim);
+        });
+    }
+    if (mine < a.n_tokens) store_columns<T, DP>(acc, scale, dq + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim);
+}
+
+// Keys [k0, k0 + 128) of one key/value head.  FAR: one chunk of the queries behind the window of a block of sinks, sums left
+// in `partial`; otherwise the queries of the block's window, after which the chunks' sums are added.
+template <typename T, int DP, bool FAR>
+__global__ __launch_bounds__(kThreads) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
+                                                                 AttentionShape a, float scale, int k_blocks, int chunk,
+                                                                 int chunks, const float* __restrict__ lse,
+                                                                 const float* __restrict__ delta, float* __restrict__ partial,
+                                                                 T* __restrict__ dk, T* __restrict__ dv) {
+    using Tl = Tiles<T, DP>;
+    __shared__ __attribute__((aligned(16))) T q_tile[kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T g_tile[kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, delta
+    const int sink_blocks = (a.sinks + kBlock - 1) / kBlock;
+    unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int c = FAR ? id % chunks : 0;
+    if (FAR) id /= chunks;
+    const int block = id % (FAR ? sink_blocks : k_blocks);
+    id /= (FAR ? sink_blocks : k_blocks);
+    const int kv_head = id % a.kv_heads;
+    const int64_t seq = id / a.kv_heads;
+    const int share = a.heads / a.kv_heads;
+    const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
+    const int length = seq_length(a, seq);
+    const int k0 = block * kBlock, w0 = k0 + wave * 32, mine = w0 + (lane_id() & 31);
+    const int near_end = min(length, k0 + kBlock + a.left);
+    const int begin = FAR ? near_end + c * chunk : max(0, k0 - a.right);
+    const int end = FAR ? min(length, begin + chunk) : near_end;
+    const int per_head = begin < end && k0 < length ? (end - begin + kTile - 1) / kTile : 0, tiles = per_head * share;
+    if (FAR && tiles == 0) return;  // the block of keys reads the chunks that its length leaves, no others
+
+    const bool kept = mine < length && (a.visible == nullptr || a.visible[seq * a.n_tokens + mine] != 0);
+    typename Tl::Frag kf, vf;
+    Tl::load_column(kf, static_cast<const T*>(k.p) + seq * k.seq + static_cast<int64_t>(mine) * k.token + kv_head * k.head, a.dim, kept);
+    Tl::load_column(vf, static_cast<const T*>(v.p) + seq * v.seq + static_cast<int64_t>(mine) * v.token + kv_head * v.head, a.dim, kept);
+    // the queries that see this lane's key: lo <= i <= hi
+    const int lo = mine - a.right, hi = !kept ? -1 : (mine < a.sinks ? length - 1 : min(mine + a.left, length - 1));
+    const bool all_kept = __all(kept);
+    // last query that sees any key of the wave
+    const int wave_last = w0 < a.sinks ? length - 1 : min(w0 + 31 + a.left, length - 1);
+
+    v16f dk_acc[DP / 32], dv_acc[DP / 32];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+
+    TileInFlight<T, DP, kTile, kThreads> q_next, g_next;
+    float stat_next = 0.0f;
+    const auto fetch = [&](int t) {
+        const int head = kv_head * share + t / per_head, i0 = begin + t % per_head * kTile;
+        q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end, a.dim);
+        g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end, a.dim);
+        const int r = i0 + (threadIdx.x & (kTile - 1));
+        if (threadIdx.x < 2 * kTile)
+            stat_next = r < end ? (threadIdx.x < kTile ? lse : delta)[(seq * a.heads + head) * a.n_tokens + r] : 0.0f;
+    };
+    if (tiles > 0) fetch(0);
+    for (int t = 0; t < tiles; ++t) {
+        const int i0 = begin + t % per_head * kTile;
+        __syncthreads();
+        q_next.store(q_tile, ~0ull);
+        g_next.store(g_tile, ~0ull);
+        if (threadIdx.x < 2 * kTile) stats[threadIdx.x / kTile][threadIdx.x % kTile] = stat_next;
+        __syncthreads();
+        if (t + 1 < tiles) fetch(t + 1);
+        if (w0 >= length || i0 + kTile <= w0 - a.right || i0 > wave_last) continue;
+        const bool whole = all_kept && i0 + kTile <= end && i0 >= w0 + 31 - a.right &&
+                           (i0 + kTile - 1 <= w0 + a.left || w0 + 32 <= a.sinks);
+        const int at = i0 + 4 * half, lo_r = lo - at, hi_r = min(hi, end - 1) - at;
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b) {
+            v16f s = Tl::rows_times(q_tile + 32 * b * Tl::LD, kf, v16f{});
+            v16f dp = Tl::rows_times(g_tile + 32 * b * Tl::LD, vf, v16f{});
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const v4f l4 = *reinterpret_cast<const v4f*>(&stats[0][32 * b + 8 * i4 + 4 * half]);
+                const v4f d4 = *reinterpret_cast<const v4f*>(&stats[1][32 * b + 8 * i4 + 4 * half]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * i4 + e, r = 32 * b + 8 * i4 + e;
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e])), ds = p * (dp[i] - d4[e]);
+                    if (!whole) {
+                        const bool seen = r >= lo_r && r <= hi_r;
+                        p = seen ? p : 0.0f;
+                        ds = seen ? ds : 0.0f;
+                    }
+                    s[i] = p;
+                    dp[i] = ds;
+                }
+            }
+            Tl::cols_times(g_tile + 32 * b * Tl::LD, s, dv_acc);
+            Tl::cols_times(q_tile + 32 * b * Tl::LD, dp, dk_acc);
+        }
+    }
+    constexpr int64_t kImage = static_cast<int64_t>(DP) * kBlock * 2;  // floats of one partial: registers x threads
+    if (FAR) {
+        float* p = partial + ((((seq * a.kv_heads + kv_head) * sink_blocks) + block) * chunks + c) * kImage + threadIdx.x;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[(2 * (dt * 16 + i)) * kThreads] = dk_acc[dt][i];
+                p[(2 * (dt * 16 + i) + 1) * kThreads] = dv_acc[dt][i];
+            }
+        return;
+    }
+    if (block < sink_blocks && near_end < length) {
+        const int filled = (length - near_end + chunk - 1) / chunk;
+        for (int n = 0; n < filled; ++n) {
+            const float* p = partial + ((((seq * a.kv_heads + kv_head) * sink_blocks) + block) * chunks + n) * kImage + threadIdx.x;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    dk_acc[dt][i] += p[(2 * (dt * 16 + i)) * kThreads];
+                    dv_acc[dt][i] += p[(2 * (dt * 16 + i) + 1) * kThreads];
+                }
+        }
+    }
+    if (__any(kept && !(all_finite(dk_acc) && all_finite(dv_acc)))) {
+        const T* kr = static_cast<const T*>(k.p) + seq * k.seq + static_cast<int64_t>(mine) * k.token + kv_head * k.head;
+        const T* vr = static_cast<const T*>(v.p) + seq * v.seq + static_cast<int64_t>(mine) * v.token + kv_head * v.head;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+        for (int h = kv_head * share; h < (kv_head + 1) * share; ++h)
+            for (int i = max(lo, 0); i <= hi; ++i) {
+                const T* qr = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(i) * q.token + h * q.head;
+                const T* gr = static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(i) * g.token + h * g.head;
+                const int64_t at = (seq * a.heads + h) * a.n_tokens + i;
+                const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, kr, a.dim), a.scale_log2, -lse[at]));
+                add_row<T, DP>(dk_acc, p * (dot_rows(gr, vr, a.dim) - delta[at]), qr, a.dim);
+                add_row<T, DP>(dv_acc, p, gr, a.dim);
+            }
+    }
+    if (mine < a.n_tokens) {
+        const int64_t row = ((seq * a.n_tokens + mine) * a.kv_heads + kv_head) * a.dim;
+        store_columns<T, DP>(dk_acc, scale, dk + row, a.dim);
+        store_columns<T, DP>(dv_acc, 1.0f, dv + row, a.dim);
+    }
+}
+
+// How the queries behind the window of the sinks' blocks are cut: enough workgroups of about the other blocks' work, at most
+// 64 chunks.
+struct FarPlan {
+    int sink_blocks, chunk, chunks;
+};
+FarPlan far_plan(int64_t n_tokens, int64_t left, int64_t sinks) {
+    FarPlan f = {0, 0, 0};
+    if (left > n_tokens) left = n_tokens;
+    if (sinks > n_tokens) sinks = n_tokens;
+    const int64_t far = n_tokens - kBlock - left;
+    if (sinks <= 0 || far <= 0) return f;
+    int64_t chunk = (left + kBlock + kTile - 1) / kTile * kTile;
+    if (chunk < 512) chunk = 512;
+    const int64_t least = (far + 63) / 64;
+    if (chunk < least) chunk = (least + kTile - 1) / kTile * kTile;
+    f.sink_blocks = static_cast<int>((sinks + kBlock - 1) / kBlock);
+    f.chunk = static_cast<int>(chunk);
+    f.chunks = static_cast<int>((far + chunk - 1) / chunk);
+    return f;
+}
+int padded_dim(int dim) { return (dim + 31) / 32 * 32; }
+
+}  // namespace
+
+int attention_shape(const char* name, int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
+                    int64_t left, int64_t right, int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
+                    AttentionShape* s);
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, TokenTensor* t);
+
+}  // namespace mvx
+
+extern "C" size_t mvx_window_attention_backward_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
+                                                                int64_t left, int64_t sinks) {
+    if (n_seqs <= 0 || n_tokens <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || left < 0) return 0;
+    const mvx::FarPlan f = mvx::far_plan(n_tokens, left, sinks);
+    const size_t rows = (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;  // delta, padded to 16 bytes
+    return (rows + static_cast<size_t>(n_seqs) * kv_heads * f.sink_blocks * f.chunks * mvx::padded_dim(dim) * mvx::kBlock * 2) *
+           sizeof(float);
+}
+
+extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                             const void* v, const int64_t* v_strides, const void* out, const float* lse,
+                                             const void* grad_out, const int64_t* grad_strides, int dtype, int64_t n_seqs,
+                                             int64_t n_tokens, int heads, int kv_heads, int dim, int64_t left, int64_t right,
+                                             int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
+                                             void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
+                                             void* stream) {
+    using namespace mvx;
+    const char* name = "mvx_window_attention_backward";
+    AttentionShape s;
+    int rc = attention_shape(name, dtype, n_seqs, n_tokens, heads, kv_heads, dim, left, right, sinks, scale, lengths, visible, &s);
+    if (rc != MVX_OK) return rc;
+    if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
+    TokenTensor qt, kt, vt, gt;
+    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, &qt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, &vt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "grad_out", grad_out, grad_strides, dtype, &gt)) != MVX_OK) return rc;
+    MVX_REQUIRE(out != nullptr && lse != nullptr && grad_q != nullptr && grad_k != nullptr && grad_v != nullptr,
+                MVX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+    MVX_REQUIRE(aligned16(out) && aligned16(grad_q) && aligned16(grad_k) && aligned16(grad_v) && aligned16(workspace),
+                MVX_ERR_INVALID_ARGUMENT, "%s: out, the gradients and the workspace must be 16-byte aligned", name);
+    const size_t need = mvx_window_attention_backward_workspace_bytes(n_seqs, n_tokens, heads, kv_heads, dim, left, sinks);
+    MVX_REQUIRE(workspace != nullptr && workspace_bytes >= need, MVX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu",
+                name, need, workspace_bytes);
+    const int64_t row = static_cast<int64_t>(heads) * dim;
+    const TokenTensor ot = {out, n_tokens * row, row, dim};
+    const int blocks = static_cast<int>((n_tokens + kBlock - 1) / kBlock);
+    const FarPlan f = far_plan(n_tokens, left, sinks);
+    MVX_REQUIRE(n_seqs <= (1 << 23) / blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23),
+                MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch", name);
+    float* delta = static_cast<float*>(workspace);
+    float* partial = delta + (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    return with_element(dtype, name, [&](auto zero) -> int {
+        using T = decltype(zero);
+        const auto launch = [&](auto dq_kernel, auto far_kernel, auto near_kernel) {
+            hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * blocks)), dim3(kThreads), 0, st, qt, kt, vt,
+                               ot, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
+            if (f.chunks > 0)
+                hipLaunchKernelGGL(far_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks * f.chunks)),
+                                   dim3(kThreads), 0, st, qt, kt, vt, gt, s, scale, blocks, f.chunk, f.chunks, lse,
+                                   const_cast<const float*>(delta), partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+            // no far queries: a chunk size that none reaches
+            hipLaunchKernelGGL(near_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
+                               vt, gt, s, scale, blocks, f.chunks > 0 ? f.chunk : 1, f.chunks, lse, const_cast<const float*>(delta),
+                               partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+        };
+        if (dim <= 32)
+            launch(window_attention_dq<T, 32>, window_attention_dkv<T, 32, true>, window_attention_dkv<T, 32, false>);
+        else if (dim <= 64)
+            launch(window_attention_dq<T, 64>, window_attention_dkv<T, 64, true>, window_attention_dkv<T, 64, false>);
+        else if (dim <= 96)
+            launch(window_attention_dq<T, 96>, window_attention_dkv<T, 96, true>, window_attention_dkv<T, 96, false>);
+        else
+            launch(window_attention_dq<T, 128>, window_attention_dkv<T, 128, true>, window_attention_dkv<T, 128, false>);
+        MVX_CHECK_LAUNCH(name);
+        return MVX_OK;
+    });
+}
