@@ -153,7 +153,8 @@ struct Tiles<float, DP> {
     }
 };
 
-// ROWS x DP tile on its way from global memory to LDS: held in registers while the previous tile is worked on.
+// ROWS x DP tile on its way from global memory to LDS, carried by THREADS neighbouring threads (the workgroup, or a wave): held
+// in registers while the previous tile is worked on.
 template <typename T, int DP, int ROWS, int THREADS>
 struct TileInFlight {
     static constexpr int VEC = Tiles<T, DP>::VEC, LD = Tiles<T, DP>::LD;
@@ -165,7 +166,7 @@ struct TileInFlight {
     __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int limit, int dim) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x + n * THREADS, r = row0 + i / PER_ROW, c = i % PER_ROW * VEC;
+            const int i = threadIdx.x % THREADS + n * THREADS, r = row0 + i / PER_ROW, c = i % PER_ROW * VEC;
             v[n] = r < limit && c < dim
                        ? *reinterpret_cast<const typename Element<T>::vec_t*>(base + static_cast<int64_t>(r) * row_stride + c)
                        : typename Element<T>::vec_t{};
@@ -175,7 +176,7 @@ struct TileInFlight {
     __device__ __forceinline__ void store(T* tile, uint64_t keep) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
+            const int i = threadIdx.x % THREADS + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
             *reinterpret_cast<typename Element<T>::vec_t*>(tile + r * LD + c) =
                 (keep >> r) & 1 ? v[n] : typename Element<T>::vec_t{};
         }

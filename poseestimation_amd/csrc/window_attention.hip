@@ -19,7 +19,7 @@ namespace {
 constexpr int kWaves = 4, kBQ = 32 * kWaves, kBK = 64;
 
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves) void window_attention(TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a,
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a,
                                                                 int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
     using Tl = Tiles<T, DP>;
     __shared__ __attribute__((aligned(16))) T k_tile[kBK * Tl::LD];
@@ -82,31 +82,39 @@ __global__ __launch_bounds__(64 * kWaves) void window_attention(TokenTensor q, T
         v16f s[kBK / 32];
 #pragma unroll
         for (int b = 0; b < kBK / 32; ++b) s[b] = Tl::rows_times(k_tile + 32 * b * Tl::LD, qf, v16f{});
-        const bool whole = keep == ~0ull && w0 + 31 < length && k0 + kBK - 1 <= w0 + a.right && (k0 >= w0 + 31 - a.left || k0 + kBK <= a.sinks);
-        float most = -kInf;
-        if (whole) {
-#pragma unroll
-            for (int b = 0; b < kBK / 32; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[b][i] *= a.scale_log2;
-                    most = fmaxf(most, s[b][i]);
-                }
-        } else {
+        const bool inside = w0 + 31 < length && k0 + kBK - 1 <= w0 + a.right;
+        const bool whole = keep == ~0ull && inside && (k0 >= w0 + 31 - a.left || k0 + kBK <= a.sinks);
+        if (!whole) {
             const int at = k0 + 4 * half;  // register i of block b is key at + 32 b + 8 (i / 4) + i % 4
-            const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
-            const uint64_t bits = keep >> (4 * half);
+            if (a.visible == nullptr && k0 >= a.sinks) {  // one range of keys: lo <= key <= hi
+                const int lo_r = hi < lo ? 1 << 30 : lo - at;  // a query at or behind the length sees none
+                const unsigned span = hi < lo ? 0 : hi - lo;
 #pragma unroll
-            for (int b = 0; b < kBK / 32; ++b)
+                for (int b = 0; b < kBK / 32; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = 32 * b + 8 * (i / 4) + i % 4;
-                    const bool seen = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1);
-                    s[b][i] = seen ? s[b][i] * a.scale_log2 : -kInf;
-                    most = fmaxf(most, s[b][i]);
-                }
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = 32 * b + 8 * (i / 4) + i % 4;
+                        s[b][i] = static_cast<unsigned>(r - lo_r) <= span ? s[b][i] : -kInf;
+                    }
+            } else {
+                const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
+                const uint64_t bits = keep >> (4 * half);
+#pragma unroll
+                for (int b = 0; b < kBK / 32; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = 32 * b + 8 * (i / 4) + i % 4;
+                        const bool seen = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1);
+                        s[b][i] = seen ? s[b][i] : -kInf;
+                    }
+            }
         }
-        most = fmaxf(both_halves_max(most), top);
+        float most = s[0][0];
+#pragma unroll
+        for (int b = 0; b < kBK / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
+        most = fmaxf(both_halves_max(most) * a.scale_log2, top);
         const float ref = most == -kInf ? 0.0f : most;
         if (__any(most > top)) {
             const float f = __builtin_amdgcn_exp2f(top - ref);  // top = -inf: 0
@@ -119,7 +127,7 @@ __global__ __launch_bounds__(64 * kWaves) void window_attention(TokenTensor q, T
         for (int b = 0; b < kBK / 32; ++b) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(s[b][i] - ref);
+                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale_log2, -ref));
                 sum += s[b][i];
             }
             Tl::cols_times(v_tile + 32 * b * Tl::LD, s[b], acc);

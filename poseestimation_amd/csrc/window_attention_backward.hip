@@ -7,9 +7,9 @@
 // fixed order and no atomics are needed (two more products of five; the result is the same in every run):
 //   1. queries in lanes, walking the tiles of keys as the forward does: delta and dq;
 //   2. keys in lanes, walking the tiles of queries that see them, over all heads that share the keys: dk and dv.
-// In the second a block of sink keys is seen by the whole rest of the sequence.  The queries beyond the block's own window
-// are therefore cut into chunks that run as workgroups of their own and leave partial sums in float32; the block itself runs
-// in a later launch and adds them in order.
+// In the second a block of sink keys is seen by the whole rest of the sequence.  The queries behind the block's own window
+// are therefore cut into chunks that a third kernel takes, between the two: a workgroup per chunk and 32 sinks, its waves
+// on queries of their own, its sum left in float32; the block of keys adds its chunks' sums in order.
 // p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.
 #include "attention_tiles.h"
 
@@ -37,7 +37,7 @@ __device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float 
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
+__global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
                                                                 TokenTensor g, AttentionShape a, float scale, int q_blocks,
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
                                                                 T* __restrict__ dq) {
@@ -140,35 +140,130 @@ __global__ __launch_bounds__(kThreads) void window_attention_dq(TokenTensor q, T
     if (mine < a.n_tokens) store_columns<T, DP>(acc, scale, dq + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim);
 }
 
-// Keys [k0, k0 + 128) of one key/value head.  FAR: one chunk of the queries behind the window of a block of sinks, sums left
-// in `partial`; otherwise the queries of the block's window, after which the chunks' sums are added.
-template <typename T, int DP, bool FAR>
-__global__ __launch_bounds__(kThreads) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
+// First query behind the window of the 128 keys from k0 on: those from here on see its sinks alone.
+__device__ __forceinline__ int window_end(const AttentionShape& a, int k0, int length) {
+    return min(length, k0 + kBlock + a.left);
+}
+// Sums of 32 sinks over one chunk of queries, in the registers' order: [register][dk, dv][lane].
+template <int DP>
+constexpr int64_t kSinkSums = static_cast<int64_t>(DP) * 32 * 2;
+template <int DP>
+__device__ __forceinline__ int64_t sink_sums(const AttentionShape& a, int64_t seq, int kv_head, int sink_block, int chunks) {
+    return ((seq * a.kv_heads + kv_head) * ((a.sinks + 31) / 32) + sink_block) * chunks * kSinkSums<DP>;
+}
+
+// One chunk of the queries behind the window of 32 sinks.  Every wave takes 32 queries of one head at a time through tiles of
+// its own (no barrier in the loop); the waves' sums are added in order at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
+                                                                   AttentionShape a, int chunk, int chunks,
+                                                                   const float* __restrict__ lse, const float* __restrict__ delta,
+                                                                   float* __restrict__ partial) {
+    using Tl = Tiles<T, DP>;
+    struct WaveTiles {
+        __attribute__((aligned(16))) T q[32 * Tl::LD];
+        __attribute__((aligned(16))) T g[32 * Tl::LD];
+        __attribute__((aligned(16))) float stats[2][32];  // lse, delta
+    };
+    __shared__ union Shared {
+        WaveTiles wave[kWaves];
+        float sums[kSinkSums<DP>];
+    } shared;
+    unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int c = id % chunks;
+    id /= chunks;
+    const int sink_blocks = (a.sinks + 31) / 32, block = id % sink_blocks;
+    id /= sink_blocks;
+    const int kv_head = id % a.kv_heads;
+    const int64_t seq = id / a.kv_heads;
+    const int share = a.heads / a.kv_heads;
+    const int lane = lane_id(), half = lane >> 5, wave = threadIdx.x >> 6;
+    const int length = seq_length(a, seq), mine = block * 32 + (lane & 31);
+    const int begin = window_end(a, block / kWaves * kBlock, length) + c * chunk, end = min(length, begin + chunk);
+    if (begin >= end) return;  // the block of keys reads the chunks that its length leaves, no others
+    const int per_head = (end - begin + 31) / 32, items = per_head * share;
+
+    const bool kept = mine < min(a.sinks, length) && (a.visible == nullptr || a.visible[seq * a.n_tokens + mine] != 0);
+    typename Tl::Frag kf, vf;
+    Tl::load_column(kf, static_cast<const T*>(k.p) + seq * k.seq + static_cast<int64_t>(mine) * k.token + kv_head * k.head, a.dim, kept);
+    Tl::load_column(vf, static_cast<const T*>(v.p) + seq * v.seq + static_cast<int64_t>(mine) * v.token + kv_head * v.head, a.dim, kept);
+    v16f dk_acc[DP / 32], dv_acc[DP / 32];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+
+    WaveTiles& tile = shared.wave[wave];
+    for (int t = wave; t < items; t += kWaves) {
+        const int head = kv_head * share + t / per_head, i0 = begin + t % per_head * 32;
+        TileInFlight<T, DP, 32, 64> q_next, g_next;
+        q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end, a.dim);
+        g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end, a.dim);
+        const int row = i0 + (lane & 31);
+        const float stat = row < end ? (half == 0 ? lse : delta)[(seq * a.heads + head) * a.n_tokens + row] : 0.0f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's reads of the last tile come before these writes
+        q_next.store(tile.q, ~0ull);
+        g_next.store(tile.g, ~0ull);
+        tile.stats[half][lane & 31] = stat;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        v16f s = Tl::rows_times(tile.q, kf, v16f{});
+        v16f dp = Tl::rows_times(tile.g, vf, v16f{});
+        const int rows = end - i0 - 4 * half;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            const v4f l4 = *reinterpret_cast<const v4f*>(&tile.stats[0][8 * i4 + 4 * half]);
+            const v4f d4 = *reinterpret_cast<const v4f*>(&tile.stats[1][8 * i4 + 4 * half]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * i4 + e;
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e])), ds = p * (dp[i] - d4[e]);
+                const bool seen = kept && 8 * i4 + e < rows;
+                s[i] = seen ? p : 0.0f;
+                dp[i] = seen ? ds : 0.0f;
+            }
+        }
+        Tl::cols_times(tile.g, s, dv_acc);
+        Tl::cols_times(tile.q, dp, dk_acc);
+    }
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) {
+        if (w == wave) {
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float* p = &shared.sums[(dt * 16 + i) * 128 + lane];
+                    p[0] = w == 0 ? dk_acc[dt][i] : p[0] + dk_acc[dt][i];
+                    p[64] = w == 0 ? dv_acc[dt][i] : p[64] + dv_acc[dt][i];
+                }
+        }
+        __syncthreads();
+    }
+    float* out = partial + sink_sums<DP>(a, seq, kv_head, block, chunks) + c * kSinkSums<DP>;
+    for (int i = threadIdx.x; i < kSinkSums<DP>; i += kThreads) out[i] = shared.sums[i];
+}
+
+// Keys [k0, k0 + 128) of one key/value head: the queries of the block's window, then the sums that window_attention_sinks
+// left for its sinks.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
                                                                  AttentionShape a, float scale, int k_blocks, int chunk,
                                                                  int chunks, const float* __restrict__ lse,
-                                                                 const float* __restrict__ delta, float* __restrict__ partial,
+                                                                 const float* __restrict__ delta, const float* __restrict__ partial,
                                                                  T* __restrict__ dk, T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
     __shared__ __attribute__((aligned(16))) T q_tile[kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) T g_tile[kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, delta
-    const int sink_blocks = (a.sinks + kBlock - 1) / kBlock;
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int c = FAR ? id % chunks : 0;
-    if (FAR) id /= chunks;
-    const int block = id % (FAR ? sink_blocks : k_blocks);
-    id /= (FAR ? sink_blocks : k_blocks);
+    const int block = id % k_blocks;
+    id /= k_blocks;
     const int kv_head = id % a.kv_heads;
     const int64_t seq = id / a.kv_heads;
     const int share = a.heads / a.kv_heads;
     const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
     const int length = seq_length(a, seq);
     const int k0 = block * kBlock, w0 = k0 + wave * 32, mine = w0 + (lane_id() & 31);
-    const int near_end = min(length, k0 + kBlock + a.left);
-    const int begin = FAR ? near_end + c * chunk : max(0, k0 - a.right);
-    const int end = FAR ? min(length, begin + chunk) : near_end;
+    const int begin = max(0, k0 - a.right), end = window_end(a, k0, length);
     const int per_head = begin < end && k0 < length ? (end - begin + kTile - 1) / kTile : 0, tiles = per_head * share;
-    if (FAR && tiles == 0) return;  // the block of keys reads the chunks that its length leaves, no others
 
     const bool kept = mine < length && (a.visible == nullptr || a.visible[seq * a.n_tokens + mine] != 0);
     typename Tl::Frag kf, vf;
@@ -232,28 +327,17 @@ __global__ __launch_bounds__(kThreads) void window_attention_dkv(TokenTensor q, 
             Tl::cols_times(q_tile + 32 * b * Tl::LD, dp, dk_acc);
         }
     }
-    constexpr int64_t kImage = static_cast<int64_t>(DP) * kBlock * 2;  // floats of one partial: registers x threads
-    if (FAR) {
-        float* p = partial + ((((seq * a.kv_heads + kv_head) * sink_blocks) + block) * chunks + c) * kImage + threadIdx.x;
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                p[(2 * (dt * 16 + i)) * kThreads] = dk_acc[dt][i];
-                p[(2 * (dt * 16 + i) + 1) * kThreads] = dv_acc[dt][i];
-            }
-        return;
-    }
-    if (block < sink_blocks && near_end < length) {
-        const int filled = (length - near_end + chunk - 1) / chunk;
-        for (int n = 0; n < filled; ++n) {
-            const float* p = partial + ((((seq * a.kv_heads + kv_head) * sink_blocks) + block) * chunks + n) * kImage + threadIdx.x;
+    const int sink_block = w0 / 32;
+    if (w0 < a.sinks && end < length) {
+        const int filled = (length - end + chunk - 1) / chunk;
+        const float* p = partial + sink_sums<DP>(a, seq, kv_head, sink_block, chunks) + lane_id();
+        for (int n = 0; n < filled; ++n, p += kSinkSums<DP>) {
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    dk_acc[dt][i] += p[(2 * (dt * 16 + i)) * kThreads];
-                    dv_acc[dt][i] += p[(2 * (dt * 16 + i) + 1) * kThreads];
+                    dk_acc[dt][i] += p[(dt * 16 + i) * 128];
+                    dv_acc[dt][i] += p[(dt * 16 + i) * 128 + 64];
                 }
         }
     }
@@ -279,22 +363,19 @@ __global__ __launch_bounds__(kThreads) void window_attention_dkv(TokenTensor q, 
     }
 }
 
-// How the queries behind the window of the sinks' blocks are cut: enough workgroups of about the other blocks' work, at most
-// 64 chunks.
+// How the queries behind the windows of the sinks are cut: chunks of 256 (two rounds of a workgroup's waves), at most 32 of
+// them, since the block of keys adds them one after the other.
 struct FarPlan {
     int sink_blocks, chunk, chunks;
 };
 FarPlan far_plan(int64_t n_tokens, int64_t left, int64_t sinks) {
-    FarPlan f = {0, 0, 0};
+    FarPlan f = {0, 1, 0};
     if (left > n_tokens) left = n_tokens;
     if (sinks > n_tokens) sinks = n_tokens;
     const int64_t far = n_tokens - kBlock - left;
     if (sinks <= 0 || far <= 0) return f;
-    int64_t chunk = (left + kBlock + kTile - 1) / kTile * kTile;
-    if (chunk < 512) chunk = 512;
-    const int64_t least = (far + 63) / 64;
-    if (chunk < least) chunk = (least + kTile - 1) / kTile * kTile;
-    f.sink_blocks = static_cast<int>((sinks + kBlock - 1) / kBlock);
+    const int64_t least = (far + 31) / 32, chunk = least <= 256 ? 256 : (least + 127) / 128 * 128;
+    f.sink_blocks = static_cast<int>((sinks + 31) / 32);
     f.chunk = static_cast<int>(chunk);
     f.chunks = static_cast<int>((far + chunk - 1) / chunk);
     return f;
@@ -315,7 +396,7 @@ extern "C" size_t mvx_window_attention_backward_workspace_bytes(int64_t n_seqs, 
     if (n_seqs <= 0 || n_tokens <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || left < 0) return 0;
     const mvx::FarPlan f = mvx::far_plan(n_tokens, left, sinks);
     const size_t rows = (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;  // delta, padded to 16 bytes
-    return (rows + static_cast<size_t>(n_seqs) * kv_heads * f.sink_blocks * f.chunks * mvx::padded_dim(dim) * mvx::kBlock * 2) *
+    return (rows + static_cast<size_t>(n_seqs) * kv_heads * f.sink_blocks * f.chunks * mvx::padded_dim(dim) * 64) *
            sizeof(float);
 }
 
@@ -355,26 +436,25 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
-        const auto launch = [&](auto dq_kernel, auto far_kernel, auto near_kernel) {
+        const auto launch = [&](auto dq_kernel, auto sinks_kernel, auto dkv_kernel) {
+            const float* d = delta;
             hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * blocks)), dim3(kThreads), 0, st, qt, kt, vt,
                                ot, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
             if (f.chunks > 0)
-                hipLaunchKernelGGL(far_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks * f.chunks)),
-                                   dim3(kThreads), 0, st, qt, kt, vt, gt, s, scale, blocks, f.chunk, f.chunks, lse,
-                                   const_cast<const float*>(delta), partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
-            // no far queries: a chunk size that none reaches
-            hipLaunchKernelGGL(near_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
-                               vt, gt, s, scale, blocks, f.chunks > 0 ? f.chunk : 1, f.chunks, lse, const_cast<const float*>(delta),
-                               partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+                hipLaunchKernelGGL(sinks_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks * f.chunks)),
+                                   dim3(kThreads), 0, st, qt, kt, vt, gt, s, f.chunk, f.chunks, lse, d, partial);
+            hipLaunchKernelGGL(dkv_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
+                               vt, gt, s, scale, blocks, f.chunk, f.chunks, lse, d, static_cast<const float*>(partial),
+                               static_cast<T*>(grad_k), static_cast<T*>(grad_v));
         };
         if (dim <= 32)
-            launch(window_attention_dq<T, 32>, window_attention_dkv<T, 32, true>, window_attention_dkv<T, 32, false>);
+            launch(window_attention_dq<T, 32>, window_attention_sinks<T, 32>, window_attention_dkv<T, 32>);
         else if (dim <= 64)
-            launch(window_attention_dq<T, 64>, window_attention_dkv<T, 64, true>, window_attention_dkv<T, 64, false>);
+            launch(window_attention_dq<T, 64>, window_attention_sinks<T, 64>, window_attention_dkv<T, 64>);
         else if (dim <= 96)
-            launch(window_attention_dq<T, 96>, window_attention_dkv<T, 96, true>, window_attention_dkv<T, 96, false>);
+            launch(window_attention_dq<T, 96>, window_attention_sinks<T, 96>, window_attention_dkv<T, 96>);
         else
-            launch(window_attention_dq<T, 128>, window_attention_dkv<T, 128, true>, window_attention_dkv<T, 128, false>);
+            launch(window_attention_dq<T, 128>, window_attention_sinks<T, 128>, window_attention_dkv<T, 128>);
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });

@@ -311,7 +311,10 @@ def test_window_attention_empty_and_extreme():
     # scores of thousands: the largest one takes all
     out = temporal.window_attention(q * 1000, k * 1000, v, (None, None))
     top = (f64(q)[0, :, 0] @ f64(k)[0, :, 0].T).argmax(-1)
-    assert torch.equal(out[0, :, 0].cpu(), v[0, :, 0].cpu()[top])
+    # every other weight is 0 and the top one some w near 1 (the exponent of 2 is score * scale less the rounded maximum), so
+    # the row is fl(fl(w v) * fl(1 / w)): three roundings of 2^-24 each, (1 + 2^-24)^3 - 1 < 3.0001 * 2^-24
+    want = v[0, :, 0].cpu()[top]
+    assert ((out[0, :, 0].cpu() - want).abs() <= 3.0001 * 2.0 ** -24 * want.abs()).all()
     scaled = temporal.window_attention(q, k, v, (5, 5), scale=0.7)
     within(scaled, *orc.attention(f64(q), f64(k), f64(v), (5, 5), 0, torch.float32, scale=0.7), "scale")
 
