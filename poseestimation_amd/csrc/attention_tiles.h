@@ -22,6 +22,15 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
 
 __device__ __forceinline__ int lane_id() { return __lane_id(); }
+// The wave's number in its workgroup, known to be the same in all lanes: what depends on it stays in scalar registers.
+__device__ __forceinline__ int same_in_all(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename T>
+__device__ __forceinline__ T* same_in_all(T* p) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    const uint64_t lo = static_cast<unsigned>(same_in_all(static_cast<int>(a))), hi = static_cast<unsigned>(same_in_all(static_cast<int>(a >> 32)));
+    return reinterpret_cast<T*>(hi << 32 | lo);
+}
+__device__ __forceinline__ int wave_id() { return same_in_all(threadIdx.x >> 6); }
 
 // max / sum over the two lanes (l, l ^ 32) that share a column: the upper half of one copy and the lower half of the other
 // are exchanged, after which the copies hold both halves' values.  (The results are copied to scalars first: a bit cast of a
@@ -48,19 +57,39 @@ __device__ __forceinline__ float both_halves_sum(float v) {
 template <typename T, int DP>
 struct Tiles;
 
+// A fragment pool holds the LDS side of 32 rows' products: filled by rows() for rows_times (16 bytes of a row per lane and
+// step) or by cols() for cols_times, and used up by the matrix instructions.  Filling and using are separate so that the reads
+// of the next product can be in flight behind the matrix instructions of this one.
 template <typename T, int DP>
 struct Tiles16 {
     typedef typename Element<T>::vec_t v8;
     static constexpr int VEC = 8;
-    static constexpr int LD = DP + 8;  // row pitch: 16-byte row reads of 8 lanes fall into different banks
+    static constexpr int STEPS = DP / 16;
+    // Tiles of 32, 64 and 128 columns are stored without padding; 16-byte chunk c of row r lies at chunk c ^ twist(r).  The
+    // twist takes 16 rows in a row (row reads: the same chunk of 16 rows) to different banks, and 4 rows in a row to different
+    // groups of 4 chunks (transposing reads: the same 4 chunks of 4 rows).  96 columns are padded by 8.
+    static constexpr bool kTwisted = (DP & (DP - 1)) == 0;
+    static constexpr int LD = kTwisted ? DP : DP + 8;
+    static __device__ __forceinline__ int twist(int r) {
+        if constexpr (DP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+        if constexpr (DP == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+        if constexpr (DP == 32) return (r >> 2) & 3;
+        return 0;
+    }
+    // index of column `col` (a multiple of 4) of row r
+    static __device__ __forceinline__ int at(int r, int col) { return r * LD + (col ^ (twist(r) << 3)); }
+
     struct Frag {
-        v8 step[DP / 16];
+        v8 step[STEPS];
+    };
+    struct Pool {
+        v8 a[STEPS];
     };
     // the lane's column: `row` points at its dim contiguous values (valid == false: zeros)
     static __device__ __forceinline__ void load_column(Frag& f, const T* row, int dim, bool valid) {
         const int half = lane_id() >> 5;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
+        for (int s = 0; s < STEPS; ++s) {
             const int d = 16 * s + 8 * half;
             f.step[s] = valid && d < dim ? *reinterpret_cast<const v8*>(row + d) : v8{};
         }
@@ -68,7 +97,7 @@ struct Tiles16 {
     static __device__ __forceinline__ float dot(const Frag& a, const Frag& b) {  // this half's share
         float r = 0.0f;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+        for (int s = 0; s < STEPS; ++s)
 #pragma unroll
             for (int e = 0; e < 8; ++e) r = fmaf(static_cast<float>(a.step[s][e]), static_cast<float>(b.step[s][e]), r);
         return r;
@@ -79,29 +108,40 @@ struct Tiles16 {
         else
             return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
-    static __device__ __forceinline__ v16f rows_times(const T* tile, const Frag& f, v16f acc) {
-        const T* p = tile + (lane_id() & 31) * LD + 8 * (lane_id() >> 5);
+    // `tile` points at a row that is a multiple of 32
+    static __device__ __forceinline__ void rows(Pool& p, const T* tile) {
+        const int r = lane_id() & 31, half = lane_id() >> 5;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) acc = mfma(*reinterpret_cast<const v8*>(p + 16 * s), f.step[s], acc);
+        for (int s = 0; s < STEPS; ++s) p.a[s] = *reinterpret_cast<const v8*>(tile + at(r, 16 * s + 8 * half));
+    }
+    static __device__ __forceinline__ void cols(Pool& p, const T* tile) {
+        typedef __attribute__((address_space(3))) v4s lds_v4s;
+        const int l = lane_id(), j = l & 15, r = 4 * (l >> 5) + (j >> 2), c = 16 * ((l >> 4) & 1) + 4 * (j & 3);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) {
+                // bit 2 of c selects the half of a chunk and is not twisted
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + at(16 * s + r, 32 * dt + c)));
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + at(16 * s + r + 8, 32 * dt + c)));
+                const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                p.a[s * (DP / 32) + dt] = __builtin_bit_cast(v8, both);
+            }
+    }
+    static __device__ __forceinline__ v16f rows_times(const Pool& p, const Frag& f) {
+        v16f acc = {};
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) acc = mfma(p.a[s], f.step[s], acc);
         return acc;
     }
-    static __device__ __forceinline__ void cols_times(const T* tile, const v16f& w, v16f (&acc)[DP / 32]) {
-        typedef __attribute__((address_space(3))) v4s lds_v4s;
-        const int l = lane_id(), j = l & 15;
-        const T* p = tile + (4 * (l >> 5) + (j >> 2)) * LD + 16 * ((l >> 4) & 1) + 4 * (j & 3);
+    static __device__ __forceinline__ void cols_times(const Pool& p, const v16f& w, v16f (&acc)[DP / 32]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             v8 b;
 #pragma unroll
             for (int e = 0; e < 8; ++e) b[e] = static_cast<T>(w[8 * s + e]);
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) {
-                const T* q = p + 16 * s * LD + 32 * dt;
-                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(q));
-                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(q + 8 * LD));
-                const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[dt] = mfma(__builtin_bit_cast(v8, both), b, acc[dt]);
-            }
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mfma(p.a[s * (DP / 32) + dt], b, acc[dt]);
         }
     }
 };
@@ -113,14 +153,19 @@ struct Tiles<f16, DP> : Tiles16<f16, DP> {};
 template <int DP>
 struct Tiles<float, DP> {
     static constexpr int VEC = 4;
+    static constexpr int STEPS = DP / 8;
     static constexpr int LD = DP + 4;
+    static __device__ __forceinline__ int at(int r, int col) { return r * LD + col; }
     struct Frag {
-        v4f step[DP / 8];  // d = 8 t + 4 half + e: the order the row reads of 16 bytes give
+        v4f step[STEPS];  // d = 8 t + 4 half + e: the order the row reads of 16 bytes give
+    };
+    struct Pool {
+        v4f a[STEPS];
     };
     static __device__ __forceinline__ void load_column(Frag& f, const float* row, int dim, bool valid) {
         const int half = lane_id() >> 5;
 #pragma unroll
-        for (int t = 0; t < DP / 8; ++t) {
+        for (int t = 0; t < STEPS; ++t) {
             const int d = 8 * t + 4 * half;
             f.step[t] = valid && d < dim ? *reinterpret_cast<const v4f*>(row + d) : v4f{};
         }
@@ -128,28 +173,42 @@ struct Tiles<float, DP> {
     static __device__ __forceinline__ float dot(const Frag& a, const Frag& b) {
         float r = 0.0f;
 #pragma unroll
-        for (int t = 0; t < DP / 8; ++t)
+        for (int t = 0; t < STEPS; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) r = fmaf(a.step[t][e], b.step[t][e], r);
         return r;
     }
-    static __device__ __forceinline__ v16f rows_times(const float* tile, const Frag& f, v16f acc) {
-        const float* p = tile + (lane_id() & 31) * LD + 4 * (lane_id() >> 5);
+    static __device__ __forceinline__ void rows(Pool& p, const float* tile) {
+        const float* q = tile + (lane_id() & 31) * LD + 4 * (lane_id() >> 5);
 #pragma unroll
-        for (int t = 0; t < DP / 8; ++t) {
-            const v4f a = *reinterpret_cast<const v4f*>(p + 8 * t);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], f.step[t][e], acc, 0, 0, 0);
-        }
-        return acc;
+        for (int t = 0; t < STEPS; ++t) p.a[t] = *reinterpret_cast<const v4f*>(q + 8 * t);
     }
-    static __device__ __forceinline__ void cols_times(const float* tile, const v16f& w, v16f (&acc)[DP / 32]) {
-        const float* p = tile + 4 * (lane_id() >> 5) * LD + (lane_id() & 31);
+    static __device__ __forceinline__ void cols(Pool& p, const float* tile) {
+        const float* q = tile + 4 * (lane_id() >> 5) * LD + (lane_id() & 31);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(p[(8 * (i / 4) + i % 4) * LD + 32 * dt], w[i], acc[dt], 0, 0, 0);
+            for (int dt = 0; dt < DP / 32; ++dt) {
+                const int n = i * (DP / 32) + dt;
+                p.a[n / 4][n % 4] = q[(8 * (i / 4) + i % 4) * LD + 32 * dt];
+            }
+    }
+    static __device__ __forceinline__ v16f rows_times(const Pool& p, const Frag& f) {
+        v16f acc = {};
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(p.a[t][e], f.step[t][e], acc, 0, 0, 0);
+        return acc;
+    }
+    static __device__ __forceinline__ void cols_times(const Pool& p, const v16f& w, v16f (&acc)[DP / 32]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) {
+                const int n = i * (DP / 32) + dt;
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(p.a[n / 4][n % 4], w[i], acc[dt], 0, 0, 0);
+            }
     }
 };
 
@@ -157,28 +216,44 @@ struct Tiles<float, DP> {
 // in registers while the previous tile is worked on.
 template <typename T, int DP, int ROWS, int THREADS>
 struct TileInFlight {
-    static constexpr int VEC = Tiles<T, DP>::VEC, LD = Tiles<T, DP>::LD;
+    static constexpr int VEC = Tiles<T, DP>::VEC;
     static constexpr int PER_ROW = DP / VEC, N = ROWS * PER_ROW / THREADS;
     static_assert(ROWS * PER_ROW % THREADS == 0, "tile must spread evenly");
     typename Element<T>::vec_t v[N];
-    // rows row0 .. row0 + ROWS - 1 of `base` (row_stride elements apart); rows from `limit` on and columns from `dim` on are
-    // zero
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int limit, int dim) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x % THREADS + n * THREADS, r = row0 + i / PER_ROW, c = i % PER_ROW * VEC;
-            v[n] = r < limit && c < dim
-                       ? *reinterpret_cast<const typename Element<T>::vec_t*>(base + static_cast<int64_t>(r) * row_stride + c)
-                       : typename Element<T>::vec_t{};
-        }
-    }
-    // rows whose bit is clear in `keep` are stored as zeros: what a hidden token holds never enters a product
-    __device__ __forceinline__ void store(T* tile, uint64_t keep) const {
+    // What a thread loads of a tile, in bytes from the tile's first value: the same in every tile.  Columns from `dim` on point
+    // behind any tile.
+    int offset[N];
+    __device__ __forceinline__ void place(int64_t row_stride, int dim) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = threadIdx.x % THREADS + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
-            *reinterpret_cast<typename Element<T>::vec_t*>(tile + r * LD + c) =
-                (keep >> r) & 1 ? v[n] : typename Element<T>::vec_t{};
+            offset[n] = c < dim ? static_cast<int>((r * row_stride + c) * sizeof(T)) : 0x7ffffff0;
+        }
+    }
+    // rows row0 .. row0 + ROWS - 1 of `base` (row_stride elements apart, at least dim; ROWS rows span less than 2^31 bytes).  A
+    // buffer that ends with row `limit` - 1 takes the bounds check: the loads behind it, and those of columns from `dim` on,
+    // give zeros.
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int limit) {
+        const int rows = max(0, min(limit - row0, ROWS));
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(same_in_all(const_cast<T*>(base + row0 * row_stride)), 0,
+                                                              same_in_all(static_cast<int>(rows * row_stride * sizeof(T))), 0x00020000);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            v[n] = __builtin_bit_cast(typename Element<T>::vec_t, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[n], 0, 0));
+    }
+    __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x % THREADS + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
+            *reinterpret_cast<typename Element<T>::vec_t*>(tile + Tiles<T, DP>::at(r, c)) = v[n];
+        }
+    }
+    // zeros in the rows whose bit is clear in `keep`: what a hidden token holds never enters a product
+    __device__ __forceinline__ void hide(uint64_t keep) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = (threadIdx.x % THREADS + n * THREADS) / PER_ROW;
+            if (!((keep >> r) & 1)) v[n] = typename Element<T>::vec_t{};
         }
     }
 };
@@ -200,14 +275,33 @@ struct AttentionShape {
 __device__ __forceinline__ int seq_length(const AttentionShape& s, int64_t seq) {
     if (s.lengths == nullptr) return s.n_tokens;
     const int64_t n = s.lengths[seq];
-    return static_cast<int>(n < 0 ? 0 : (n < s.n_tokens ? n : s.n_tokens));
+    return same_in_all(static_cast<int>(n < 0 ? 0 : (n < s.n_tokens ? n : s.n_tokens)));
 }
-// Bit r: token first + r exists (below `length`) and is visible.  Every lane of the wave takes part.
-__device__ __forceinline__ uint64_t tokens_kept(const AttentionShape& s, int64_t seq, int first, int length) {
+// Whether token first + lane exists (below `length`) and is visible; its ballot has a bit per token of a tile.
+__device__ __forceinline__ bool token_kept(const AttentionShape& s, int64_t seq, int first, int length) {
     const int j = first + lane_id();
-    bool keep = j < length;
-    if (s.visible != nullptr && keep) keep = s.visible[seq * s.n_tokens + j] != 0;
-    return __ballot(keep);
+    return j < length && (s.visible == nullptr || s.visible[seq * s.n_tokens + j] != 0);
+}
+
+// The tiles of `step` keys that the queries [q0, q0 + n) see: first those of the sinks, then the window.
+struct KeyTiles {
+    int count, sinks, first;
+    __device__ __forceinline__ int key0(int t, int step) const { return (t < sinks ? t : first + t - sinks) * step; }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const AttentionShape& s, int q0, int n, int length, int step) {
+    KeyTiles k = {0, 0, 0};
+    if (q0 >= length) return k;
+    k.first = max(0, q0 - s.left) / step;
+    k.sinks = min((min(s.sinks, length) + step - 1) / step, k.first);
+    k.count = min(q0 + n - 1 + s.right, length - 1) / step + 1 - k.first + k.sinks;
+    return k;
+}
+// Whether any / each of the queries [w0, w0 + 32) sees any / each of the keys [k0, k0 + n), hidden ones aside.
+__device__ __forceinline__ bool sees_any(const AttentionShape& s, int w0, int k0, int n, int length) {
+    return w0 < length && k0 <= min(w0 + 31 + s.right, length - 1) && (k0 + n > w0 - s.left || k0 < s.sinks);
+}
+__device__ __forceinline__ bool sees_all(const AttentionShape& s, int w0, int k0, int n, int length) {
+    return w0 + 31 < length && k0 + n <= min(w0 + s.right + 1, length) && (k0 >= w0 + 31 - s.left || k0 + n <= s.sinks);
 }
 
 // ---- pairs one by one -------------------------------------------------------------------------------------------------

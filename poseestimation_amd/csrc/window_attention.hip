@@ -17,13 +17,14 @@ namespace mvx {
 namespace {
 
 constexpr int kWaves = 4, kBQ = 32 * kWaves, kBK = 64;
+constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2^15
 
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a,
                                                                 int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
     using Tl = Tiles<T, DP>;
-    __shared__ __attribute__((aligned(16))) T k_tile[kBK * Tl::LD];
-    __shared__ __attribute__((aligned(16))) T v_tile[kBK * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T k_tile[2][kBK * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T v_tile[2][kBK * Tl::LD];
     // heads that share keys, then blocks of queries, are neighbours on one XCD
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int share = a.heads / a.kv_heads;
@@ -34,7 +35,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
     const int kv_head = id % a.kv_heads;
     const int64_t seq = id / a.kv_heads;
     const int head = kv_head * share + in_group;
-    const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
+    const int half = lane_id() >> 5, wave = wave_id();
     const int length = seq_length(a, seq);
     const int q0 = block * kBQ, mine = q0 + wave * 32 + (lane_id() & 31);
 
@@ -46,13 +47,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
 
     // the keys this lane's query sees: j <= hi and (j >= lo or j < sinks)
     const int hi = mine < length ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
-    int tiles = 0, sink_tiles = 0, first_tile = 0;
-    if (q0 < length) {
-        first_tile = max(0, q0 - a.left) / kBK;
-        tiles = min(q0 + kBQ - 1 + a.right, length - 1) / kBK + 1 - first_tile;
-        sink_tiles = min((min(a.sinks, length) + kBK - 1) / kBK, first_tile);
-        tiles += sink_tiles;
-    }
+    const KeyTiles tiles = key_tiles(a, q0, kBQ, length, kBK);
     const int w0 = q0 + wave * 32;  // the wave's first query
 
     v16f acc[DP / 32];
@@ -61,30 +56,53 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
     float top = -kInf, sum = 0.0f;
 
     TileInFlight<T, DP, kBK, 64 * kWaves> k_next, v_next;
-    if (tiles > 0) {
-        const int k0 = (sink_tiles > 0 ? 0 : first_tile) * kBK;
-        k_next.load(kb, k.token, k0, length, a.dim);
-        v_next.load(vb, v.token, k0, length, a.dim);
-    }
-    for (int t = 0; t < tiles; ++t) {
-        const int k0 = (t < sink_tiles ? t : first_tile + t - sink_tiles) * kBK;
-        const uint64_t keep = tokens_kept(a, seq, k0, length);
-        __syncthreads();  // the previous tile is read
-        k_next.store(k_tile, keep);
-        v_next.store(v_tile, keep);
-        __syncthreads();
-        if (t + 1 < tiles) {
-            const int n0 = (t + 1 < sink_tiles ? t + 1 : first_tile + t + 1 - sink_tiles) * kBK;
-            k_next.load(kb, k.token, n0, length, a.dim);
-            v_next.load(vb, v.token, n0, length, a.dim);
+    k_next.place(k.token, a.dim);
+    v_next.place(v.token, a.dim);
+    bool kept_next = false;
+    const auto fetch = [&](int t) {
+        const int k0 = tiles.key0(t, kBK);
+        k_next.load(kb, k.token, k0, length);
+        v_next.load(vb, v.token, k0, length);
+        kept_next = token_kept(a, seq, k0, length);
+    };
+    const auto put = [&](int t) {
+        const uint64_t keep = __ballot(kept_next);
+        if (a.visible != nullptr && keep != ~0ull) {
+            k_next.hide(keep);
+            v_next.hide(keep);
         }
-        if (w0 >= length || k0 > min(w0 + 31 + a.right, length - 1) || (k0 + kBK <= w0 - a.left && k0 >= a.sinks)) continue;
-        v16f s[kBK / 32];
-#pragma unroll
-        for (int b = 0; b < kBK / 32; ++b) s[b] = Tl::rows_times(k_tile + 32 * b * Tl::LD, qf, v16f{});
-        const bool inside = w0 + 31 < length && k0 + kBK - 1 <= w0 + a.right;
-        const bool whole = keep == ~0ull && inside && (k0 >= w0 + 31 - a.left || k0 + kBK <= a.sinks);
-        if (!whole) {
+        k_next.store(k_tile[t & 1]);
+        v_next.store(v_tile[t & 1]);
+        return keep;
+    };
+    uint64_t keep = 0, keep_next = 0;
+    if (tiles.count > 0) {
+        fetch(0);
+        keep_next = put(0);
+    }
+    if (tiles.count > 1) fetch(1);
+    for (int t = 0; t < tiles.count; ++t) {
+        keep = keep_next;
+        __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
+        if (t + 1 < tiles.count) keep_next = put(t + 1);
+        if (t + 2 < tiles.count) fetch(t + 2);
+        const int k0 = tiles.key0(t, kBK);
+        if (!sees_any(a, w0, k0, kBK, length)) continue;
+        const T *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+        // the wave's blocks of 32 keys, from b0 to b1: at the ends of the window it may need one of the two
+        const int b0 = sees_any(a, w0, k0, 32, length) ? 0 : 1, b1 = sees_any(a, w0, k0 + 32, 32, length) ? 2 : 1;
+        v16f s[2];
+        typename Tl::Pool pool, more;
+        Tl::rows(pool, kt + 32 * b0 * Tl::LD);
+        if (b1 - b0 == 2) {
+            Tl::rows(more, kt + 32 * Tl::LD);
+            s[0] = Tl::rows_times(pool, qf);
+            s[1] = Tl::rows_times(more, qf);
+        } else {
+            s[b0] = Tl::rows_times(pool, qf);
+            s[1 - b0] = v16f{};
+        }
+        if (keep != ~0ull || !sees_all(a, w0, k0, kBK, length)) {
             const int at = k0 + 4 * half;  // register i of block b is key at + 32 b + 8 (i / 4) + i % 4
             if (a.visible == nullptr && k0 >= a.sinks) {  // one range of keys: lo <= key <= hi
                 const int lo_r = hi < lo ? 1 << 30 : lo - at;  // a query at or behind the length sees none
@@ -114,23 +132,28 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
         for (int b = 0; b < kBK / 32; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
-        most = fmaxf(both_halves_max(most) * a.scale_log2, top);
-        const float ref = most == -kInf ? 0.0f : most;
-        if (__any(most > top)) {
-            const float f = __builtin_amdgcn_exp2f(top - ref);  // top = -inf: 0
+        most = both_halves_max(most) * a.scale_log2;
+        // the reference moves only when a score passes it by 2^kSlack: weights stay below that, and what they lose in the
+        // rounding to 16 bits is relative
+        if (__any(most > top + kSlack)) {
+            const float next = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - (next == -kInf ? 0.0f : next));
             sum *= f;
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= f;
-            top = most;
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= f;  // top = -inf: 0
+            top = next;
         }
+        const float ref = top == -kInf ? 0.0f : top;
+        Tl::cols(pool, vt + 32 * b0 * Tl::LD);
 #pragma unroll
-        for (int b = 0; b < kBK / 32; ++b) {
+        for (int b = 0; b < 2; ++b) {
+            if (b < b0 || b >= b1) continue;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale_log2, -ref));
                 sum += s[b][i];
             }
-            Tl::cols_times(v_tile + 32 * b * Tl::LD, s[b], acc);
+            Tl::cols_times(pool, s[b], acc);
+            if (b == 0 && b1 == 2) Tl::cols(pool, vt + 32 * Tl::LD);
         }
     }
     sum = both_halves_sum(sum);
@@ -192,12 +215,17 @@ int attention_shape(const char* name, int dtype, int64_t n_seqs, int64_t n_token
     return MVX_OK;
 }
 
-int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, TokenTensor* t) {
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_tokens,
+                     int dim, TokenTensor* t) {
     MVX_REQUIRE(p != nullptr && strides != nullptr, MVX_ERR_INVALID_ARGUMENT, "%s: null pointer (%s)", name, what);
     const int64_t vec = 16 / element_bytes(dtype);
     MVX_REQUIRE(aligned16(p) && strides[0] % vec == 0 && strides[1] % vec == 0 && strides[2] % vec == 0, MVX_ERR_INVALID_ARGUMENT,
                 "%s: %s must be 16-byte aligned in its base and strides", name, what);
-    *t = {p, strides[0], strides[1], strides[2]};
+    // a tile of 64 tokens is addressed with 31 bits, and bounded by its last token
+    MVX_REQUIRE(n_tokens == 1 || (strides[1] >= dim && strides[1] < (1LL << 31) / 64 / element_bytes(dtype)), MVX_ERR_INVALID_ARGUMENT,
+                "%s: tokens of %s must be at least a head (%d values) and less than 2^25 bytes apart, got %lld values", name, what,
+                dim, (long long)strides[1]);
+    *t = {p, strides[0], n_tokens == 1 ? dim : strides[1], strides[2]};
     return MVX_OK;
 }
 
@@ -214,9 +242,9 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     if (rc != MVX_OK) return rc;
     if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
     TokenTensor qt, kt, vt;
-    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, &qt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, &kt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, &vt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, n_tokens, dim, &qt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_tokens, dim, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_tokens, dim, &vt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && aligned16(out), MVX_ERR_INVALID_ARGUMENT, "%s: out is null or not 16-byte aligned", name);
     const int q_blocks = static_cast<int>((n_tokens + kBQ - 1) / kBQ);
     MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",

@@ -42,8 +42,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
                                                                 T* __restrict__ dq) {
     using Tl = Tiles<T, DP>;
-    __shared__ __attribute__((aligned(16))) T k_tile[kTile * Tl::LD];
-    __shared__ __attribute__((aligned(16))) T v_tile[kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T v_tile[2][kTile * Tl::LD];
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int share = a.heads / a.kv_heads;
     const int in_group = id % share;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     const int kv_head = id % a.kv_heads;
     const int64_t seq = id / a.kv_heads;
     const int head = kv_head * share + in_group;
-    const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
+    const int half = lane_id() >> 5, wave = wave_id();
     const int length = seq_length(a, seq);
     const int q0 = block * kBlock, w0 = q0 + wave * 32, mine = w0 + (lane_id() & 31);
 
@@ -75,56 +75,68 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     if (mine < a.n_tokens && half == 0) delta[at_row] = my_delta;
 
     const int hi = live ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
-    int tiles = 0, sink_tiles = 0, first_tile = 0;
-    if (q0 < length) {
-        first_tile = max(0, q0 - a.left) / kTile;
-        tiles = min(q0 + kBlock - 1 + a.right, length - 1) / kTile + 1 - first_tile;
-        sink_tiles = min((min(a.sinks, length) + kTile - 1) / kTile, first_tile);
-        tiles += sink_tiles;
-    }
+    const KeyTiles tiles = key_tiles(a, q0, kBlock, length, kTile);
     v16f acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
 
     TileInFlight<T, DP, kTile, kThreads> k_next, v_next;
-    if (tiles > 0) {
-        const int k0 = (sink_tiles > 0 ? 0 : first_tile) * kTile;
-        k_next.load(kb, k.token, k0, length, a.dim);
-        v_next.load(vb, v.token, k0, length, a.dim);
-    }
-    for (int t = 0; t < tiles; ++t) {
-        const int k0 = (t < sink_tiles ? t : first_tile + t - sink_tiles) * kTile;
-        const uint64_t keep = tokens_kept(a, seq, k0, length);
-        __syncthreads();
-        k_next.store(k_tile, keep);
-        v_next.store(v_tile, keep);
-        __syncthreads();
-        if (t + 1 < tiles) {
-            const int n0 = (t + 1 < sink_tiles ? t + 1 : first_tile + t + 1 - sink_tiles) * kTile;
-            k_next.load(kb, k.token, n0, length, a.dim);
-            v_next.load(vb, v.token, n0, length, a.dim);
+    k_next.place(k.token, a.dim);
+    v_next.place(v.token, a.dim);
+    bool kept_next = false;
+    const auto fetch = [&](int t) {
+        const int k0 = tiles.key0(t, kTile);
+        k_next.load(kb, k.token, k0, length);
+        v_next.load(vb, v.token, k0, length);
+        kept_next = token_kept(a, seq, k0, length);
+    };
+    const auto put = [&](int t) {
+        const uint64_t keep = __ballot(kept_next);
+        if (a.visible != nullptr && keep != ~0ull) {
+            k_next.hide(keep);
+            v_next.hide(keep);
         }
-        if (w0 >= length || k0 > min(w0 + 31 + a.right, length - 1) || (k0 + kTile <= w0 - a.left && k0 >= a.sinks)) continue;
-        const bool whole = keep == ~0ull && w0 + 31 < length && k0 + kTile - 1 <= w0 + a.right &&
-                           (k0 >= w0 + 31 - a.left || k0 + kTile <= a.sinks);
+        k_next.store(k_tile[t & 1]);
+        v_next.store(v_tile[t & 1]);
+        return keep;
+    };
+    uint64_t keep = 0, keep_next = 0;
+    if (tiles.count > 0) {
+        fetch(0);
+        keep_next = put(0);
+    }
+    if (tiles.count > 1) fetch(1);
+    for (int t = 0; t < tiles.count; ++t) {
+        keep = keep_next;
+        __syncthreads();
+        if (t + 1 < tiles.count) keep_next = put(t + 1);
+        if (t + 2 < tiles.count) fetch(t + 2);
+        const int k0 = tiles.key0(t, kTile);
+        const T *kt = k_tile[t & 1], *vt = v_tile[t & 1];
         const int at = k0 + 4 * half;
         const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
         const uint64_t bits = keep >> (4 * half);
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b) {
-            v16f s = Tl::rows_times(k_tile + 32 * b * Tl::LD, qf, v16f{});
-            const v16f dp = Tl::rows_times(v_tile + 32 * b * Tl::LD, gf, v16f{});
+            if (!sees_any(a, w0, k0 + 32 * b, 32, length)) continue;
+            const bool whole = static_cast<unsigned>(keep >> (32 * b)) == ~0u && sees_all(a, w0, k0 + 32 * b, 32, length);
+            typename Tl::Pool pool, more;
+            Tl::rows(pool, kt + 32 * b * Tl::LD);
+            Tl::rows(more, vt + 32 * b * Tl::LD);
+            v16f s = Tl::rows_times(pool, qf);
+            Tl::cols(pool, kt + 32 * b * Tl::LD);
+            const v16f dp = Tl::rows_times(more, gf);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float ds = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -my_lse)) * (dp[i] - my_delta);
-                if (whole) {
-                    s[i] = ds;
-                } else {
+            for (int i = 0; i < 16; ++i)
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -my_lse)) * (dp[i] - my_delta);
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     const int r = 32 * b + 8 * (i / 4) + i % 4;
-                    s[i] = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1) ? ds : 0.0f;
+                    s[i] = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1) ? s[i] : 0.0f;
                 }
             }
-            Tl::cols_times(k_tile + 32 * b * Tl::LD, s, acc);
+            Tl::cols_times(pool, s, acc);
         }
     }
     if (__any(live && !all_finite(acc))) {
@@ -177,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
     const int kv_head = id % a.kv_heads;
     const int64_t seq = id / a.kv_heads;
     const int share = a.heads / a.kv_heads;
-    const int lane = lane_id(), half = lane >> 5, wave = threadIdx.x >> 6;
+    const int lane = lane_id(), half = lane >> 5, wave = wave_id();
     const int length = seq_length(a, seq), mine = block * 32 + (lane & 31);
     const int begin = window_end(a, block / kWaves * kBlock, length) + c * chunk, end = min(length, begin + chunk);
     if (begin >= end) return;  // the block of keys reads the chunks that its length leaves, no others
@@ -192,20 +204,27 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
     for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
 
     WaveTiles& tile = shared.wave[wave];
+    TileInFlight<T, DP, 32, 64> q_next, g_next;
+    q_next.place(q.token, a.dim);
+    g_next.place(g.token, a.dim);
     for (int t = wave; t < items; t += kWaves) {
         const int head = kv_head * share + t / per_head, i0 = begin + t % per_head * 32;
-        TileInFlight<T, DP, 32, 64> q_next, g_next;
-        q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end, a.dim);
-        g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end, a.dim);
+        q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end);
+        g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end);
         const int row = i0 + (lane & 31);
         const float stat = row < end ? (half == 0 ? lse : delta)[(seq * a.heads + head) * a.n_tokens + row] : 0.0f;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's reads of the last tile come before these writes
-        q_next.store(tile.q, ~0ull);
-        g_next.store(tile.g, ~0ull);
+        q_next.store(tile.q);
+        g_next.store(tile.g);
         tile.stats[half][lane & 31] = stat;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        v16f s = Tl::rows_times(tile.q, kf, v16f{});
-        v16f dp = Tl::rows_times(tile.g, vf, v16f{});
+        typename Tl::Pool pool, more;
+        Tl::rows(pool, tile.q);
+        Tl::rows(more, tile.g);
+        v16f s = Tl::rows_times(pool, kf);
+        Tl::cols(pool, tile.g);
+        v16f dp = Tl::rows_times(more, vf);
+        Tl::cols(more, tile.q);
         const int rows = end - i0 - 4 * half;
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
@@ -220,8 +239,8 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
                 dp[i] = seen ? ds : 0.0f;
             }
         }
-        Tl::cols_times(tile.g, s, dv_acc);
-        Tl::cols_times(tile.q, dp, dk_acc);
+        Tl::cols_times(pool, s, dv_acc);
+        Tl::cols_times(more, dp, dk_acc);
     }
     __syncthreads();
     for (int w = 0; w < kWaves; ++w) {
@@ -250,16 +269,16 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
                                                                  const float* __restrict__ delta, const float* __restrict__ partial,
                                                                  T* __restrict__ dk, T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
-    __shared__ __attribute__((aligned(16))) T q_tile[kTile * Tl::LD];
-    __shared__ __attribute__((aligned(16))) T g_tile[kTile * Tl::LD];
-    __shared__ __attribute__((aligned(16))) float stats[2][kTile];  // lse, delta
+    __shared__ __attribute__((aligned(16))) T q_tile[2][kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) T g_tile[2][kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse, delta
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int block = id % k_blocks;
     id /= k_blocks;
     const int kv_head = id % a.kv_heads;
     const int64_t seq = id / a.kv_heads;
     const int share = a.heads / a.kv_heads;
-    const int half = lane_id() >> 5, wave = threadIdx.x >> 6;
+    const int half = lane_id() >> 5, wave = wave_id();
     const int length = seq_length(a, seq);
     const int k0 = block * kBlock, w0 = k0 + wave * 32, mine = w0 + (lane_id() & 31);
     const int begin = max(0, k0 - a.right), end = window_end(a, k0, length);
@@ -280,51 +299,69 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
     for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
 
     TileInFlight<T, DP, kTile, kThreads> q_next, g_next;
+    q_next.place(q.token, a.dim);
+    g_next.place(g.token, a.dim);
     float stat_next = 0.0f;
     const auto fetch = [&](int t) {
         const int head = kv_head * share + t / per_head, i0 = begin + t % per_head * kTile;
-        q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end, a.dim);
-        g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end, a.dim);
+        q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end);
+        g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end);
         const int r = i0 + (threadIdx.x & (kTile - 1));
         if (threadIdx.x < 2 * kTile)
             stat_next = r < end ? (threadIdx.x < kTile ? lse : delta)[(seq * a.heads + head) * a.n_tokens + r] : 0.0f;
     };
-    if (tiles > 0) fetch(0);
+    const auto put = [&](int t) {
+        q_next.store(q_tile[t & 1]);
+        g_next.store(g_tile[t & 1]);
+        if (threadIdx.x < 2 * kTile) stats[t & 1][threadIdx.x / kTile][threadIdx.x % kTile] = stat_next;
+    };
+    if (tiles > 0) {
+        fetch(0);
+        put(0);
+    }
+    if (tiles > 1) fetch(1);
     for (int t = 0; t < tiles; ++t) {
         const int i0 = begin + t % per_head * kTile;
         __syncthreads();
-        q_next.store(q_tile, ~0ull);
-        g_next.store(g_tile, ~0ull);
-        if (threadIdx.x < 2 * kTile) stats[threadIdx.x / kTile][threadIdx.x % kTile] = stat_next;
-        __syncthreads();
-        if (t + 1 < tiles) fetch(t + 1);
-        if (w0 >= length || i0 + kTile <= w0 - a.right || i0 > wave_last) continue;
-        const bool whole = all_kept && i0 + kTile <= end && i0 >= w0 + 31 - a.right &&
-                           (i0 + kTile - 1 <= w0 + a.left || w0 + 32 <= a.sinks);
+        if (t + 1 < tiles) put(t + 1);
+        if (t + 2 < tiles) fetch(t + 2);
+        if (w0 >= length) continue;
+        const T *qt = q_tile[t & 1], *gt = g_tile[t & 1];
         const int at = i0 + 4 * half, lo_r = lo - at, hi_r = min(hi, end - 1) - at;
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b) {
-            v16f s = Tl::rows_times(q_tile + 32 * b * Tl::LD, kf, v16f{});
-            v16f dp = Tl::rows_times(g_tile + 32 * b * Tl::LD, vf, v16f{});
+            const int r0 = i0 + 32 * b;  // the block's first query
+            if (r0 >= end || r0 + 32 <= w0 - a.right || r0 > wave_last) continue;
+            const bool whole = all_kept && r0 + 32 <= end && r0 >= w0 + 31 - a.right && (r0 + 31 <= w0 + a.left || w0 + 32 <= a.sinks);
+            typename Tl::Pool pool, more;
+            Tl::rows(pool, qt + 32 * b * Tl::LD);
+            Tl::rows(more, gt + 32 * b * Tl::LD);
+            v16f s = Tl::rows_times(pool, kf);
+            Tl::cols(pool, gt + 32 * b * Tl::LD);
+            v16f dp = Tl::rows_times(more, vf);
+            Tl::cols(more, qt + 32 * b * Tl::LD);
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
-                const v4f l4 = *reinterpret_cast<const v4f*>(&stats[0][32 * b + 8 * i4 + 4 * half]);
-                const v4f d4 = *reinterpret_cast<const v4f*>(&stats[1][32 * b + 8 * i4 + 4 * half]);
+                const v4f l4 = *reinterpret_cast<const v4f*>(&stats[t & 1][0][32 * b + 8 * i4 + 4 * half]);
+                const v4f d4 = *reinterpret_cast<const v4f*>(&stats[t & 1][1][32 * b + 8 * i4 + 4 * half]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 4 * i4 + e, r = 32 * b + 8 * i4 + e;
-                    float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e])), ds = p * (dp[i] - d4[e]);
-                    if (!whole) {
-                        const bool seen = r >= lo_r && r <= hi_r;
-                        p = seen ? p : 0.0f;
-                        ds = seen ? ds : 0.0f;
-                    }
-                    s[i] = p;
-                    dp[i] = ds;
+                    const int i = 4 * i4 + e;
+                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e]));
+                    dp[i] = s[i] * (dp[i] - d4[e]);
                 }
             }
-            Tl::cols_times(g_tile + 32 * b * Tl::LD, s, dv_acc);
-            Tl::cols_times(q_tile + 32 * b * Tl::LD, dp, dk_acc);
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 32 * b + 8 * (i / 4) + i % 4;
+                    const bool seen = r >= lo_r && r <= hi_r;
+                    s[i] = seen ? s[i] : 0.0f;
+                    dp[i] = seen ? dp[i] : 0.0f;
+                }
+            }
+            Tl::cols_times(pool, s, dv_acc);
+            Tl::cols_times(more, dp, dk_acc);
         }
     }
     const int sink_block = w0 / 32;
@@ -387,7 +424,8 @@ int padded_dim(int dim) { return (dim + 31) / 32 * 32; }
 int attention_shape(const char* name, int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
                     int64_t left, int64_t right, int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
                     AttentionShape* s);
-int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, TokenTensor* t);
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_tokens,
+                     int dim, TokenTensor* t);
 
 }  // namespace mvx
 
@@ -414,10 +452,10 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     if (rc != MVX_OK) return rc;
     if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
     TokenTensor qt, kt, vt, gt;
-    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, &qt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, &kt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, &vt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "grad_out", grad_out, grad_strides, dtype, &gt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, n_tokens, dim, &qt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_tokens, dim, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_tokens, dim, &vt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "grad_out", grad_out, grad_strides, dtype, n_tokens, dim, &gt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && lse != nullptr && grad_q != nullptr && grad_k != nullptr && grad_v != nullptr,
                 MVX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
     MVX_REQUIRE(aligned16(out) && aligned16(grad_q) && aligned16(grad_k) && aligned16(grad_v) && aligned16(workspace),

@@ -223,9 +223,11 @@ def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum
 
 def _tokens(t):
     """`t` (batch, tokens, heads, head_dim) as the attention kernels read it: last axis contiguous, base and strides multiples
-    of 16 bytes.  Other layouts are copied."""
-    vec = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st % vec == 0 or size == 1 for st, size in zip(t.stride()[:3], t.shape)):
+    of 16 bytes, tokens a head or more and less than 2^25 bytes apart.  Other layouts are copied."""
+    size = t.element_size()
+    vec = 16 // size
+    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st % vec == 0 or n == 1 for st, n in zip(t.stride()[:3], t.shape))
+            and (t.shape[1] <= 1 or t.shape[3] <= t.stride(1) < (1 << 25) // size)):
         return t
     c = t.contiguous()
     return c if c.data_ptr() % 16 == 0 else c.clone()
