@@ -217,8 +217,7 @@ struct Tiles<float, DP> {
 template <typename T, int DP, int ROWS, int THREADS>
 struct TileInFlight {
     static constexpr int VEC = Tiles<T, DP>::VEC;
-    static constexpr int PER_ROW = DP / VEC, N = ROWS * PER_ROW / THREADS;
-    static_assert(ROWS * PER_ROW % THREADS == 0, "tile must spread evenly");
+    static constexpr int PER_ROW = DP / VEC, ALL = ROWS * PER_ROW, N = (ALL + THREADS - 1) / THREADS;
     typename Element<T>::vec_t v[N];
     // What a thread loads of a tile, in bytes from the tile's first value: the same in every tile.  Columns from `dim` on point
     // behind any tile.
@@ -227,7 +226,7 @@ struct TileInFlight {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = threadIdx.x % THREADS + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
-            offset[n] = c < dim ? static_cast<int>((r * row_stride + c) * sizeof(T)) : 0x7ffffff0;
+            offset[n] = c < dim && i < ALL ? static_cast<int>((r * row_stride + c) * sizeof(T)) : 0x7ffffff0;
         }
     }
     // rows row0 .. row0 + ROWS - 1 of `base` (row_stride elements apart, at least dim; ROWS rows span less than 2^31 bytes).  A
@@ -245,7 +244,8 @@ struct TileInFlight {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = threadIdx.x % THREADS + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
-            *reinterpret_cast<typename Element<T>::vec_t*>(tile + Tiles<T, DP>::at(r, c)) = v[n];
+            if (ALL % THREADS == 0 || i < ALL)
+                *reinterpret_cast<typename Element<T>::vec_t*>(tile + Tiles<T, DP>::at(r, c)) = v[n];
         }
     }
     // zeros in the rows whose bit is clear in `keep`: what a hidden token holds never enters a product
@@ -257,6 +257,24 @@ struct TileInFlight {
         }
     }
 };
+
+// Stores the lane's column of a 32 x DP block of sums: times `factor`, the first `dim` values of `row`.
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float factor, T* row, int dim) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const int half = lane_id() >> 5;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = 32 * dt + 8 * b + 4 * half;
+            if (d >= dim) continue;
+            vec4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[dt][4 * b + e] * factor);
+            *reinterpret_cast<vec4*>(row + d) = w;
+        }
+}
 
 // What the attention entry points share.
 struct TokenTensor {
@@ -298,10 +316,10 @@ __device__ __forceinline__ KeyTiles key_tiles(const AttentionShape& s, int q0, i
 }
 // Whether any / each of the queries [w0, w0 + 32) sees any / each of the keys [k0, k0 + n), hidden ones aside.
 __device__ __forceinline__ bool sees_any(const AttentionShape& s, int w0, int k0, int n, int length) {
-    return w0 < length && k0 <= min(w0 + 31 + s.right, length - 1) && (k0 + n > w0 - s.left || k0 < s.sinks);
+    return (w0 < length) & (k0 <= min(w0 + 31 + s.right, length - 1)) & ((k0 + n > w0 - s.left) | (k0 < s.sinks));
 }
 __device__ __forceinline__ bool sees_all(const AttentionShape& s, int w0, int k0, int n, int length) {
-    return w0 + 31 < length && k0 + n <= min(w0 + s.right + 1, length) && (k0 >= w0 + 31 - s.left || k0 + n <= s.sinks);
+    return (w0 + 32 <= length) & (k0 + n <= min(w0 + s.right + 1, length)) & ((k0 >= w0 + 31 - s.left) | (k0 + n <= s.sinks));
 }
 
 // ---- pairs one by one -------------------------------------------------------------------------------------------------

@@ -19,10 +19,12 @@ namespace {
 constexpr int kWaves = 4, kBQ = 32 * kWaves, kBK = 64;
 constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2^15
 
+// The registers are cut for two waves per SIMD where they suffice: with one, a long prompt of heads of 128 took 1.8 times as long.
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a,
-                                                                int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
+    TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
     using Tl = Tiles<T, DP>;
+    constexpr int DT = DP / 32;
     __shared__ __attribute__((aligned(16))) T k_tile[2][kBK * Tl::LD];
     __shared__ __attribute__((aligned(16))) T v_tile[2][kBK * Tl::LD];
     // heads that share keys, then blocks of queries, are neighbours on one XCD
@@ -37,24 +39,21 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
     const int head = kv_head * share + in_group;
     const int half = lane_id() >> 5, wave = wave_id();
     const int length = seq_length(a, seq);
-    const int q0 = block * kBQ, mine = q0 + wave * 32 + (lane_id() & 31);
+    const int q0 = block * kBQ, w0 = q0 + wave * 32;  // the workgroup's and the wave's first query
 
     const T* kb = static_cast<const T*>(k.p) + seq * k.seq + kv_head * k.head;
     const T* vb = static_cast<const T*>(v.p) + seq * v.seq + kv_head * v.head;
-    typename Tl::Frag qf;
-    Tl::load_column(qf, static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head, a.dim,
-                    mine < length);
-
-    // the keys this lane's query sees: j <= hi and (j >= lo or j < sinks)
+    const T* qb = static_cast<const T*>(q.p) + seq * q.seq + head * q.head;
+    const int mine = w0 + (lane_id() & 31);  // this lane's query, and the keys it sees: j <= hi and (j >= lo or j < sinks)
     const int hi = mine < length ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
-    const KeyTiles tiles = key_tiles(a, q0, kBQ, length, kBK);
-    const int w0 = q0 + wave * 32;  // the wave's first query
-
-    v16f acc[DP / 32];
+    typename Tl::Frag qf;
+    Tl::load_column(qf, qb + static_cast<int64_t>(mine) * q.token, a.dim, mine < length);
+    v16f acc[DT];
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
     float top = -kInf, sum = 0.0f;
 
+    const KeyTiles tiles = key_tiles(a, q0, kBQ, length, kBK);
     TileInFlight<T, DP, kBK, 64 * kWaves> k_next, v_next;
     k_next.place(k.token, a.dim);
     v_next.place(v.token, a.dim);
@@ -87,85 +86,67 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
         if (t + 1 < tiles.count) keep_next = put(t + 1);
         if (t + 2 < tiles.count) fetch(t + 2);
         const int k0 = tiles.key0(t, kBK);
-        if (!sees_any(a, w0, k0, kBK, length)) continue;
         const T *kt = k_tile[t & 1], *vt = v_tile[t & 1];
-        // the wave's blocks of 32 keys, from b0 to b1: at the ends of the window it may need one of the two
-        const int b0 = sees_any(a, w0, k0, 32, length) ? 0 : 1, b1 = sees_any(a, w0, k0 + 32, 32, length) ? 2 : 1;
-        v16f s[2];
-        typename Tl::Pool pool, more;
-        Tl::rows(pool, kt + 32 * b0 * Tl::LD);
-        if (b1 - b0 == 2) {
-            Tl::rows(more, kt + 32 * Tl::LD);
-            s[0] = Tl::rows_times(pool, qf);
-            s[1] = Tl::rows_times(more, qf);
-        } else {
-            s[b0] = Tl::rows_times(pool, qf);
-            s[1 - b0] = v16f{};
-        }
-        if (keep != ~0ull || !sees_all(a, w0, k0, kBK, length)) {
-            const int at = k0 + 4 * half;  // register i of block b is key at + 32 b + 8 (i / 4) + i % 4
-            if (a.visible == nullptr && k0 >= a.sinks) {  // one range of keys: lo <= key <= hi
-                const int lo_r = hi < lo ? 1 << 30 : lo - at;  // a query at or behind the length sees none
-                const unsigned span = hi < lo ? 0 : hi - lo;
-#pragma unroll
-                for (int b = 0; b < kBK / 32; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = 32 * b + 8 * (i / 4) + i % 4;
-                        s[b][i] = static_cast<unsigned>(r - lo_r) <= span ? s[b][i] : -kInf;
-                    }
-            } else {
+#pragma unroll 1  // two copies need more registers than two waves per SIMD have
+        for (int b = 0; b < kBK; b += 32) {
+            if (!sees_any(a, w0, k0 + b, 32, length)) continue;
+            typename Tl::Pool pool;
+            Tl::rows(pool, kt + b * Tl::LD);
+            v16f s = Tl::rows_times(pool, qf);
+            Tl::cols(pool, vt + b * Tl::LD);
+            const unsigned kept = static_cast<unsigned>(keep >> b);
+            if (kept != ~0u || !sees_all(a, w0, k0 + b, 32, length)) {
+                const int at = k0 + b + 4 * half;  // register i is key at + 8 (i / 4) + i % 4
                 const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
-                const uint64_t bits = keep >> (4 * half);
+                if (a.visible == nullptr && k0 + b >= a.sinks) {  // one range of keys, lo <= key <= hi
+                    const int from = hi < lo ? 1 << 30 : lo_r;  // a query at or behind the length sees none
+                    const unsigned span = hi < lo ? 0 : hi - lo;
 #pragma unroll
-                for (int b = 0; b < kBK / 32; ++b)
+                    for (int i = 0; i < 16; ++i)
+                        s[i] = static_cast<unsigned>(8 * (i / 4) + i % 4 - from) <= span ? s[i] : -kInf;
+                } else {
+                    const unsigned bits = kept >> (4 * half);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int r = 32 * b + 8 * (i / 4) + i % 4;
-                        const bool seen = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1);
-                        s[b][i] = seen ? s[b][i] : -kInf;
+                        const int r = 8 * (i / 4) + i % 4;
+                        const bool seen = (r <= hi_r) & ((r >= lo_r) | (r < sink_r)) & ((bits >> r) & 1);
+                        s[i] = seen ? s[i] : -kInf;
                     }
+                }
             }
-        }
-        float most = s[0][0];
+            float most = s[0];
 #pragma unroll
-        for (int b = 0; b < kBK / 32; ++b)
+            for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+            most = both_halves_max(most) * a.scale_log2;
+            // The reference of the exponents moves only when a score passes it by 2^kSlack: weights stay below that, and what
+            // they lose in the rounding to 16 bits is relative.
+            if (__any(most > top + kSlack)) {
+                const float next = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - (next == -kInf ? 0.0f : next));
+                sum *= f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
-        most = both_halves_max(most) * a.scale_log2;
-        // the reference moves only when a score passes it by 2^kSlack: weights stay below that, and what they lose in the
-        // rounding to 16 bits is relative
-        if (__any(most > top + kSlack)) {
-            const float next = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - (next == -kInf ? 0.0f : next));
-            sum *= f;
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= f;  // top = -inf: 0
-            top = next;
-        }
-        const float ref = top == -kInf ? 0.0f : top;
-        Tl::cols(pool, vt + 32 * b0 * Tl::LD);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            if (b < b0 || b >= b1) continue;
+                for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;  // top = -inf: 0
+                top = next;
+            }
+            const float ref = top == -kInf ? 0.0f : top;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale_log2, -ref));
-                sum += s[b][i];
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -ref));
+                sum += s[i];
             }
-            Tl::cols_times(pool, s[b], acc);
-            if (b == 0 && b1 == 2) Tl::cols(pool, vt + 32 * Tl::LD);
+            Tl::cols_times(pool, s, acc);
         }
     }
     sum = both_halves_sum(sum);
     if (__any(mine < length && !(all_finite(acc) && sum < kInf))) {
-        const T* qr = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head;
+        const T* qr = qb + static_cast<int64_t>(mine) * q.token;
         top = -kInf;
         sum = 0.0f;
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
-        for_seen_keys(a, seq, lo, hi, [&](int j) { top = fmaxf(top, dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2); });
-        // every score a NaN: a reference of 0 keeps the row apart from one that sees nothing
-        if (hi >= 0) for_seen_keys(a, seq, lo, hi, [&](int) { top = fmaxf(top, -3.0e38f); });
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
+        // every score a NaN: a finite reference keeps the row apart from one that sees nothing
+        for_seen_keys(a, seq, lo, hi, [&](int j) {
+            top = fmaxf(fmaxf(top, -3.0e38f), dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2);
+        });
         for_seen_keys(a, seq, lo, hi, [&](int j) {
             const float p = __builtin_amdgcn_exp2f(dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2 - top);
             sum += p;
@@ -174,22 +155,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
     }
     if (mine >= a.n_tokens) return;
     const bool none = top == -kInf;
-    const float inv = none ? 0.0f : 1.0f / sum;
     if (lse != nullptr && half == 0)
         lse[(seq * a.heads + head) * a.n_tokens + mine] = none ? 0.0f : top + __builtin_amdgcn_logf(sum);  // log2
-    T* o = out + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim;
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int d = 32 * dt + 8 * b + 4 * half;
-            if (d >= a.dim) continue;
-            vec4 w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(none ? 0.0f : acc[dt][4 * b + e] * inv);
-            *reinterpret_cast<vec4*>(o + d) = w;
-        }
+    store_columns<T, DP>(acc, none ? 0.0f : 1.0f / sum, out + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim);
 }
 
 }  // namespace

@@ -20,23 +20,6 @@ namespace {
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlock = 32 * kWaves, kTile = 64;
 
 template <typename T, int DP>
-__device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float factor, T* row, int dim) {
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-    const int half = lane_id() >> 5;
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int d = 32 * dt + 8 * b + 4 * half;
-            if (d >= dim) continue;
-            vec4 w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[dt][4 * b + e] * factor);
-            *reinterpret_cast<vec4*>(row + d) = w;
-        }
-}
-
-template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
                                                                 TokenTensor g, AttentionShape a, float scale, int q_blocks,
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
@@ -116,16 +99,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
         const int at = k0 + 4 * half;
         const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
         const uint64_t bits = keep >> (4 * half);
-#pragma unroll
+#pragma unroll 1  // two copies need more registers than two waves per SIMD have
         for (int b = 0; b < kTile / 32; ++b) {
             if (!sees_any(a, w0, k0 + 32 * b, 32, length)) continue;
             const bool whole = static_cast<unsigned>(keep >> (32 * b)) == ~0u && sees_all(a, w0, k0 + 32 * b, 32, length);
-            typename Tl::Pool pool, more;
+            typename Tl::Pool pool;
             Tl::rows(pool, kt + 32 * b * Tl::LD);
-            Tl::rows(more, vt + 32 * b * Tl::LD);
             v16f s = Tl::rows_times(pool, qf);
+            Tl::rows(pool, vt + 32 * b * Tl::LD);
+            const v16f dp = Tl::rows_times(pool, gf);
             Tl::cols(pool, kt + 32 * b * Tl::LD);
-            const v16f dp = Tl::rows_times(more, gf);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -my_lse)) * (dp[i] - my_delta);
@@ -133,7 +116,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 32 * b + 8 * (i / 4) + i % 4;
-                    s[i] = r <= hi_r && (r >= lo_r || r < sink_r) && ((bits >> r) & 1) ? s[i] : 0.0f;
+                    s[i] = (r <= hi_r) & ((r >= lo_r) | (r < sink_r)) & ((bits >> r) & 1) ? s[i] : 0.0f;
                 }
             }
             Tl::cols_times(pool, s, acc);
@@ -328,18 +311,17 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
         if (w0 >= length) continue;
         const T *qt = q_tile[t & 1], *gt = g_tile[t & 1];
         const int at = i0 + 4 * half, lo_r = lo - at, hi_r = min(hi, end - 1) - at;
-#pragma unroll
+#pragma unroll 1  // two copies need more registers than two waves per SIMD have
         for (int b = 0; b < kTile / 32; ++b) {
             const int r0 = i0 + 32 * b;  // the block's first query
             if (r0 >= end || r0 + 32 <= w0 - a.right || r0 > wave_last) continue;
             const bool whole = all_kept && r0 + 32 <= end && r0 >= w0 + 31 - a.right && (r0 + 31 <= w0 + a.left || w0 + 32 <= a.sinks);
-            typename Tl::Pool pool, more;
+            typename Tl::Pool pool;
             Tl::rows(pool, qt + 32 * b * Tl::LD);
-            Tl::rows(more, gt + 32 * b * Tl::LD);
             v16f s = Tl::rows_times(pool, kf);
+            Tl::rows(pool, gt + 32 * b * Tl::LD);
+            v16f dp = Tl::rows_times(pool, vf);
             Tl::cols(pool, gt + 32 * b * Tl::LD);
-            v16f dp = Tl::rows_times(more, vf);
-            Tl::cols(more, qt + 32 * b * Tl::LD);
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
                 const v4f l4 = *reinterpret_cast<const v4f*>(&stats[t & 1][0][32 * b + 8 * i4 + 4 * half]);
@@ -361,7 +343,8 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
                 }
             }
             Tl::cols_times(pool, s, dv_acc);
-            Tl::cols_times(more, dp, dk_acc);
+            Tl::cols(pool, qt + 32 * b * Tl::LD);
+            Tl::cols_times(pool, dp, dk_acc);
         }
     }
     const int sink_block = w0 / 32;
