@@ -167,12 +167,25 @@ extern "C" int mvx_rotate_positions(const void* q, const int64_t* q_strides, int
     const int64_t rows = n_seqs * n_tokens;
     MVX_REQUIRE(n_seqs <= 0x7fffffffLL && n_tokens <= 0x7fffffffLL && rows <= 0x7fffffffLL, MVX_ERR_UNSUPPORTED,
                 "%s: more than 2^31 - 1 tokens", name);
-    for (int a = 0, i = 0; a < n_axes; ++a)
-        for (int j = 0; j < sections[a]; ++j, ++i) {
-            const double e = shared_spectrum ? static_cast<double>(i) / static_cast<double>(pairs)
-                                             : static_cast<double>(j) / static_cast<double>(sections[a]);
-            table.turns[i] = pow(base, -e) / 6.283185307179586476925286766559;
-        }
+    // The powers cost more host time than the launch: a thread keeps those of its last sections and base.
+    thread_local struct {
+        double base = 0.0;
+        int n_axes = 0, shared = 0, end[kMaxAxes] = {};
+        double turns[kMaxPairs];
+    } last;
+    bool same = last.base == base && last.n_axes == n_axes && last.shared == (shared_spectrum != 0);
+    for (int a = 0; a < n_axes; ++a) same = same && last.end[a] == table.end[a];
+    if (!same) {
+        for (int a = 0, i = 0; a < n_axes; ++a)
+            for (int j = 0; j < sections[a]; ++j, ++i) {
+                const double e = shared_spectrum ? static_cast<double>(i) / static_cast<double>(pairs)
+                                                 : static_cast<double>(j) / static_cast<double>(sections[a]);
+                last.turns[i] = pow(base, -e) / 6.283185307179586476925286766559;
+            }
+        last.base = base, last.n_axes = n_axes, last.shared = shared_spectrum != 0;
+        for (int a = 0; a < n_axes; ++a) last.end[a] = table.end[a];
+    }
+    for (int i = 0; i < pairs; ++i) table.turns[i] = last.turns[i];
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
         constexpr int VEC = Element<T>::vec;

@@ -183,17 +183,18 @@ int attention_shape(const char* name, int dtype, int64_t n_seqs, int64_t n_token
     return MVX_OK;
 }
 
-int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_tokens,
-                     int dim, TokenTensor* t) {
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_seqs,
+                     int64_t n_tokens, int heads, int dim, TokenTensor* t) {
     MVX_REQUIRE(p != nullptr && strides != nullptr, MVX_ERR_INVALID_ARGUMENT, "%s: null pointer (%s)", name, what);
+    // the stride of an axis of length 1 is never used, whatever it says
+    *t = {p, n_seqs > 1 ? strides[0] : 0, n_tokens > 1 ? strides[1] : dim, heads > 1 ? strides[2] : 0};
     const int64_t vec = 16 / element_bytes(dtype);
-    MVX_REQUIRE(aligned16(p) && strides[0] % vec == 0 && strides[1] % vec == 0 && strides[2] % vec == 0, MVX_ERR_INVALID_ARGUMENT,
+    MVX_REQUIRE(aligned16(p) && t->seq % vec == 0 && t->token % vec == 0 && t->head % vec == 0, MVX_ERR_INVALID_ARGUMENT,
                 "%s: %s must be 16-byte aligned in its base and strides", name, what);
     // a tile of 64 tokens is addressed with 31 bits, and bounded by its last token
-    MVX_REQUIRE(n_tokens == 1 || (strides[1] >= dim && strides[1] < (1LL << 31) / 64 / element_bytes(dtype)), MVX_ERR_INVALID_ARGUMENT,
+    MVX_REQUIRE(t->token >= dim && t->token < (1LL << 31) / 64 / element_bytes(dtype), MVX_ERR_INVALID_ARGUMENT,
                 "%s: tokens of %s must be at least a head (%d values) and less than 2^25 bytes apart, got %lld values", name, what,
-                dim, (long long)strides[1]);
-    *t = {p, strides[0], n_tokens == 1 ? dim : strides[1], strides[2]};
+                dim, (long long)t->token);
     return MVX_OK;
 }
 
@@ -210,9 +211,9 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     if (rc != MVX_OK) return rc;
     if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
     TokenTensor qt, kt, vt;
-    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, n_tokens, dim, &qt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_tokens, dim, &kt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_tokens, dim, &vt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, n_seqs, n_tokens, heads, dim, &qt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && aligned16(out), MVX_ERR_INVALID_ARGUMENT, "%s: out is null or not 16-byte aligned", name);
     const int q_blocks = static_cast<int>((n_tokens + kBQ - 1) / kBQ);
     MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",

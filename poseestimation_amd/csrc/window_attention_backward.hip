@@ -407,8 +407,8 @@ int padded_dim(int dim) { return (dim + 31) / 32 * 32; }
 int attention_shape(const char* name, int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
                     int64_t left, int64_t right, int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
                     AttentionShape* s);
-int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_tokens,
-                     int dim, TokenTensor* t);
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_seqs,
+                     int64_t n_tokens, int heads, int dim, TokenTensor* t);
 
 }  // namespace mvx
 
@@ -435,10 +435,10 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     if (rc != MVX_OK) return rc;
     if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
     TokenTensor qt, kt, vt, gt;
-    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, n_tokens, dim, &qt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_tokens, dim, &kt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_tokens, dim, &vt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "grad_out", grad_out, grad_strides, dtype, n_tokens, dim, &gt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "q", q, q_strides, dtype, n_seqs, n_tokens, heads, dim, &qt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "grad_out", grad_out, grad_strides, dtype, n_seqs, n_tokens, heads, dim, &gt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && lse != nullptr && grad_q != nullptr && grad_k != nullptr && grad_v != nullptr,
                 MVX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
     MVX_REQUIRE(aligned16(out) && aligned16(grad_q) && aligned16(grad_k) && aligned16(grad_v) && aligned16(workspace),

@@ -251,8 +251,8 @@ int check_cache(const char* name, int dtype, int64_t n_seqs, int kv_heads, int d
 
 }  // namespace
 
-int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_tokens,
-                     int dim, TokenTensor* t);
+int attention_tensor(const char* name, const char* what, const void* p, const int64_t* strides, int dtype, int64_t n_seqs,
+                     int64_t n_tokens, int heads, int dim, TokenTensor* t);
 
 }  // namespace mvx
 
@@ -322,8 +322,8 @@ extern "C" int mvx_window_cache_fill(const void* k, const int64_t* k_strides, co
     MVX_REQUIRE(n_tokens >= 0, MVX_ERR_INVALID_ARGUMENT, "%s: bad n_tokens=%lld", name, (long long)n_tokens);
     if (n_seqs == 0 || n_tokens == 0) return MVX_OK;
     TokenTensor kt, vt;
-    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_tokens, dim, &kt)) != MVX_OK) return rc;
-    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_tokens, dim, &vt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &kt)) != MVX_OK) return rc;
+    if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
     MVX_REQUIRE(lengths != nullptr && k_cache != nullptr && v_cache != nullptr && aligned16(k_cache) && aligned16(v_cache),
                 MVX_ERR_INVALID_ARGUMENT, "%s: lengths or a cache is null, or a cache is not 16-byte aligned", name);
     const int slots = static_cast<int>(window + sinks);

@@ -14,6 +14,7 @@ stream of the tensors' device and can be captured into a graph.  layer_norm, rot
 differentiable (once) by backward kernels whose sums run in a fixed order.
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -23,7 +24,11 @@ from poseestimation_amd import _cabi
 
 _DTYPES = {torch.float32: _cabi.F32, torch.bfloat16: _cabi.BF16, torch.float16: _cabi.F16}
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
-_Strides = ctypes.c_int64 * 3
+
+
+# The smallest calls of this module take a few microseconds of GPU time, less than the checks of their arguments would when
+# made one by one.  Each entry point therefore accepts the usual case by one cheap condition and looks for what is wrong, and
+# how to say it, only where that fails.
 
 
 def _check(t, name, like=None, like_name=None):
@@ -41,16 +46,51 @@ def _check(t, name, like=None, like_name=None):
             _cabi.same_device(like, like_name, **{name: t})
 
 
-def _run(device, what, entry, *args):
-    """Calls a C entry point on torch's current stream of `device`."""
-    index = device.index
+def _check_qkv(q, k, v):
+    try:
+        if q.is_cuda and q.dtype in _DTYPES and q.dtype == k.dtype == v.dtype and q.get_device() == k.get_device() == v.get_device():
+            return
+    except AttributeError:
+        pass
+    _check(q, "q")
+    _check(k, "k", q, "q")
+    _check(v, "v", q, "q")
+
+
+_lib = None
+
+
+def _run(index, what, entry, *args):
+    """Calls the C entry point `entry` on torch's current stream of device `index`."""
+    global _lib
+    if _lib is None:
+        _lib = _cabi.load()
+    entry = getattr(_lib, entry)
     if index == torch.cuda.current_device():
         status = entry(*args, _cabi.raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = entry(*args, _cabi.raw_stream(index))
     if status != _cabi.MVX_OK:
         _cabi.check(status, what)
+
+
+def _pointer(t):
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _int64s(values):
+    return (ctypes.c_int64 * 4)(*values)
+
+
+@functools.lru_cache(maxsize=1024)
+def _int32s(values):
+    return (ctypes.c_int32 * len(values))(*values)
+
+
+def _strides(t):
+    return _int64s(t.stride())
 
 
 def _workspace(n_bytes, device):
@@ -60,7 +100,7 @@ def _workspace(n_bytes, device):
 # ---- layer norm --------------------------------------------------------------------------------------------------------
 
 
-def _norm_shapes(x, weight, bias, eps):
+def _norm_check(x, weight, bias, eps):
     _check(x, "x")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("x must have a last axis of at least one value, got shape %s" % (tuple(x.shape),))
@@ -76,7 +116,16 @@ def _norm_shapes(x, weight, bias, eps):
             raise ValueError("%s must have shape %s, got %s" % (name, tuple(x.shape[-1:]), tuple(p.shape)))
         if p.dtype not in (x.dtype, torch.float32) or p.dtype != param.dtype:
             raise ValueError("weight and bias must both be float32 or both of x's type %s, got %s for %s" % (x.dtype, p.dtype, name))
-    return param is not None and param.dtype == torch.float32
+
+
+def _norm_usual(x, weight, bias, eps):
+    """Whether this is a call with both parameters of x's type in which nothing is wrong."""
+    try:
+        width = x.shape[-1]
+        return (x.is_cuda and weight.dtype == bias.dtype == x.dtype and x.dtype in _DTYPES and weight.shape == bias.shape == (width,)
+                and x.get_device() == weight.get_device() == bias.get_device() and width > 0 and 0.0 <= eps < math.inf)
+    except (AttributeError, IndexError, TypeError):
+        return False
 
 
 def _norm_run(x, weight, bias, eps, param_f32, want_stats):
@@ -87,9 +136,8 @@ def _norm_run(x, weight, bias, eps, param_f32, want_stats):
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if want_stats else None
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
-    _run(x.device, "mvx_layer_norm", _cabi.load().mvx_layer_norm, x.data_ptr(),
-         weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None, _DTYPES[x.dtype],
-         int(param_f32), rows, width, eps, y.data_ptr(), stats.data_ptr() if want_stats else None)
+    _run(x.get_device(), "layer_norm", "mvx_layer_norm", x.data_ptr(), _pointer(weight), _pointer(bias), _DTYPES[x.dtype],
+         param_f32, rows, width, eps, y.data_ptr(), _pointer(stats))
     return x, y, stats
 
 
@@ -114,13 +162,12 @@ class _LayerNorm(torch.autograd.Function):
         grad_x = torch.empty_like(x) if need_x else None
         grad_w = torch.empty(width, dtype=weight.dtype, device=x.device) if need_w else None
         grad_b = torch.empty(ctx.bias_like[0], dtype=ctx.bias_like[1], device=x.device) if need_b else None
-        lib = _cabi.load()
         dtype = _DTYPES[x.dtype]
-        ws = _workspace(lib.mvx_layer_norm_backward_workspace_bytes(dtype, rows, width), x.device) if need_w or need_b else None
-        _run(x.device, "mvx_layer_norm_backward", lib.mvx_layer_norm_backward, grad_y.data_ptr(), x.data_ptr(),
-             weight.data_ptr() if weight is not None else None, stats.data_ptr(), dtype, int(ctx.param_f32), rows, width,
-             grad_x.data_ptr() if need_x else None, grad_w.data_ptr() if need_w else None,
-             grad_b.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
+        n_bytes = _cabi.load().mvx_layer_norm_backward_workspace_bytes(dtype, rows, width) if need_w or need_b else 0
+        ws = _workspace(n_bytes, x.device)
+        _run(x.get_device(), "layer_norm", "mvx_layer_norm_backward", grad_y.data_ptr(), x.data_ptr(), _pointer(weight),
+             stats.data_ptr(), dtype, ctx.param_f32, rows, width, _pointer(grad_x), _pointer(grad_w), _pointer(grad_b),
+             ws.data_ptr(), ws.numel())
         return grad_x, grad_w, grad_b, None, None
 
 
@@ -129,10 +176,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     weight and bias (width,) are of x's type or float32 (both alike); None stands for ones and zeros.  Differentiable with
     respect to x, weight and bias."""
-    param_f32 = _norm_shapes(x, weight, bias, eps)
-    if _cabi.needs_grad(x, weight, bias):
+    param_f32 = 0
+    if not _norm_usual(x, weight, bias, eps):
+        _norm_check(x, weight, bias, eps)
+        param = weight if weight is not None else bias
+        param_f32 = int(param is not None and param.dtype == torch.float32)
+    if torch.is_grad_enabled() and _cabi.needs_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps), param_f32)
-    return _norm_run(x, weight, bias, float(eps), param_f32, False)[1]
+    return _norm_run(x, weight, bias, eps, param_f32, False)[1]
 
 
 # ---- rotary positions --------------------------------------------------------------------------------------------------
@@ -140,20 +191,20 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 def _rotate_run(q, k, positions, sections, base, shared, pairs, inverse):
     b, n, heads, dim = q.shape
-    q = q if q.stride(-1) == 1 else q.contiguous()
+    if q.stride(3) != 1:
+        q = q.contiguous()
     q_out = torch.empty((b, n, heads, dim), dtype=q.dtype, device=q.device)
+    k_out, k_args = None, (None, None, 0)
     if k is not None:
-        k = k if k.stride(-1) == 1 else k.contiguous()
+        if k.stride(3) != 1:
+            k = k.contiguous()
         k_heads = k.shape[2]
         k_out = torch.empty((b, n, k_heads, dim), dtype=q.dtype, device=q.device)
-        k_args = (k.data_ptr(), _Strides(*k.stride()[:3]), k_heads)
-    else:
-        k_out, k_args = None, (None, None, 0)
+        k_args = (k.data_ptr(), _strides(k), k_heads)
     n_axes = len(sections)
-    _run(q.device, "mvx_rotate_positions", _cabi.load().mvx_rotate_positions, q.data_ptr(), _Strides(*q.stride()[:3]), heads,
-         *k_args, _DTYPES[q.dtype], b, n, dim, positions.data_ptr(), _POSITION_TYPES[positions.dtype],
-         n * n_axes if positions.dim() == 3 else 0, n_axes, (ctypes.c_int32 * n_axes)(*sections), base, shared, pairs, inverse,
-         q_out.data_ptr(), k_out.data_ptr() if k_out is not None else None)
+    _run(q.get_device(), "rotate_positions", "mvx_rotate_positions", q.data_ptr(), _strides(q), heads, *k_args, _DTYPES[q.dtype], b, n,
+         dim, positions.data_ptr(), _POSITION_TYPES[positions.dtype], n * n_axes if positions.dim() == 3 else 0, n_axes,
+         _int32s(sections), base, shared, pairs, inverse, q_out.data_ptr(), _pointer(k_out))
     return q_out, k_out
 
 
@@ -179,15 +230,7 @@ class _Rotate(torch.autograd.Function):
         return grad_q if need_q else None, grad_k if need_k else None, None, None, None, None, None
 
 
-def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum=False, pairs=False):
-    """Rotary positions with several axes: returns (q, k) with the first 2 * sum(sections) values of every head turned pair by
-    pair, the rest copied.  Both come from one launch; k may be None.
-
-    q (batch, tokens, heads, head_dim), k (batch, tokens, kv_heads, head_dim); positions (batch, tokens, axes) or
-    (tokens, axes), int32, int64, float32 or float64; sections: the pairs of each axis (1 to 4 axes, at most 128 pairs).  Pair
-    i turns by position[axis] * base ** -e, with e its place in the axis' section over the section's pairs or, with
-    shared_spectrum, i over all pairs.  Pairs are (i, i + all pairs), or neighbours (2i, 2i + 1) with pairs=True.  Angles are
-    float64, so positions of millions keep their place.  Differentiable with respect to q and k."""
+def _rotate_check(q, k, positions, sections, base):
     _check(q, "q")
     if q.dim() != 4:
         raise ValueError("q must have shape (batch, tokens, heads, head_dim), got %s" % (tuple(q.shape),))
@@ -195,7 +238,6 @@ def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum
         _check(k, "k", q, "q")
         if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
             raise ValueError("k must have shape (%d, %d, kv_heads, %d), got %s" % (q.shape[0], q.shape[1], q.shape[3], tuple(k.shape)))
-    sections = tuple(int(s) for s in sections)
     if not torch.is_tensor(positions):
         raise TypeError("positions must be a torch tensor, got %s" % type(positions).__name__)
     _cabi.forward_only("rotate_positions (positions)", positions)
@@ -211,9 +253,37 @@ def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum
         raise ValueError("q and k must have at least one head")
     if not (math.isfinite(base) and base > 0):
         raise ValueError("base must be positive and finite, got %r" % (base,))
+
+
+def _rotate_usual(q, k, positions, sections, base):
+    """Whether this is a call with q, k and positions of every sequence in which nothing is wrong."""
+    try:
+        b, n, heads, dim = q.shape
+        kb, kn, k_heads, k_dim = k.shape
+        pb, pn, axes = positions.shape
+        return (q.is_cuda and q.dtype in _DTYPES and q.dtype == k.dtype and positions.dtype in _POSITION_TYPES
+                and not positions.requires_grad and q.get_device() == k.get_device() == positions.get_device()
+                and b == kb == pb and n == kn == pn and dim == k_dim and heads > 0 and k_heads > 0 and axes == len(sections)
+                and 1 <= axes <= 4 and min(sections) >= 0 and 1 <= sum(sections) <= dim // 2 and 0.0 < base < math.inf)
+    except (AttributeError, TypeError, ValueError):
+        return False
+
+
+def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum=False, pairs=False):
+    """Rotary positions with several axes: returns (q, k) with the first 2 * sum(sections) values of every head turned pair by
+    pair, the rest copied.  Both come from one launch; k may be None.
+
+    q (batch, tokens, heads, head_dim), k (batch, tokens, kv_heads, head_dim); positions (batch, tokens, axes) or
+    (tokens, axes), int32, int64, float32 or float64; sections: the pairs of each axis (1 to 4 axes, at most 128 pairs).  Pair
+    i turns by position[axis] * base ** -e, with e its place in the axis' section over the section's pairs or, with
+    shared_spectrum, i over all pairs.  Pairs are (i, i + all pairs), or neighbours (2i, 2i + 1) with pairs=True.  Angles are
+    float64, so positions of millions keep their place.  Differentiable with respect to q and k."""
+    sections = tuple(map(int, sections))
+    if not _rotate_usual(q, k, positions, sections, base):
+        _rotate_check(q, k, positions, sections, base)
     positions = positions.contiguous()
     how = (sections, float(base), int(bool(shared_spectrum)), int(bool(pairs)))
-    if _cabi.needs_grad(q, k):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotate.apply(q, k, positions, *how)
     return _rotate_run(q, k, positions, *how, 0)
 
@@ -224,17 +294,16 @@ def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum
 def _tokens(t):
     """`t` (batch, tokens, heads, head_dim) as the attention kernels read it: last axis contiguous, base and strides multiples
     of 16 bytes, tokens a head or more and less than 2^25 bytes apart.  Other layouts are copied."""
+    aligned = t.data_ptr() % 16 == 0
+    if aligned and t.is_contiguous() and t.shape[2] * t.shape[3] < 1 << 22:
+        return t
     size = t.element_size()
     vec = 16 // size
-    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st % vec == 0 or n == 1 for st, n in zip(t.stride()[:3], t.shape))
+    if (aligned and t.stride(3) == 1 and all(st % vec == 0 or n == 1 for st, n in zip(t.stride()[:3], t.shape))
             and (t.shape[1] <= 1 or t.shape[3] <= t.stride(1) < (1 << 25) // size)):
         return t
     c = t.contiguous()
     return c if c.data_ptr() % 16 == 0 else c.clone()
-
-
-def _strides(t):
-    return _Strides(*(st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape)))
 
 
 def _window_run(q, k, v, lengths, visible, how, want_lse):
@@ -242,10 +311,9 @@ def _window_run(q, k, v, lengths, visible, how, want_lse):
     b, n, heads, dim = q.shape
     out = torch.empty((b, n, heads, dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, heads, n), dtype=torch.float32, device=q.device) if want_lse else None
-    _run(q.device, "mvx_window_attention", _cabi.load().mvx_window_attention, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-         v.data_ptr(), _strides(v), _DTYPES[q.dtype], b, n, heads, k.shape[2], dim, *how,
-         lengths.data_ptr() if lengths is not None else None, visible.data_ptr() if visible is not None else None, out.data_ptr(),
-         lse.data_ptr() if want_lse else None)
+    _run(q.get_device(), "window_attention", "mvx_window_attention", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
+         v.data_ptr(), _strides(v), _DTYPES[q.dtype], b, n, heads, k.shape[2], dim, *how, _pointer(lengths), _pointer(visible),
+         out.data_ptr(), _pointer(lse))
     return q, k, v, out, lse
 
 
@@ -268,13 +336,11 @@ class _WindowAttention(torch.autograd.Function):
         grad_q = torch.empty((b, n, heads, dim), dtype=q.dtype, device=q.device)
         grad_k = torch.empty((b, n, kv_heads, dim), dtype=q.dtype, device=q.device)
         grad_v = torch.empty_like(grad_k)
-        lib = _cabi.load()
-        ws = _workspace(lib.mvx_window_attention_backward_workspace_bytes(b, n, heads, kv_heads, dim, left, sinks), q.device)
-        _run(q.device, "mvx_window_attention_backward", lib.mvx_window_attention_backward, q.data_ptr(), _strides(q), k.data_ptr(),
-             _strides(k), v.data_ptr(), _strides(v), out.data_ptr(), lse.data_ptr(), grad.data_ptr(), _strides(grad),
-             _DTYPES[q.dtype], b, n, heads, kv_heads, dim, left, right, sinks, scale,
-             lengths.data_ptr() if lengths is not None else None, visible.data_ptr() if visible is not None else None,
-             grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(), ws.data_ptr(), ws.numel())
+        ws = _workspace(_cabi.load().mvx_window_attention_backward_workspace_bytes(b, n, heads, kv_heads, dim, left, sinks), q.device)
+        _run(q.get_device(), "window_attention", "mvx_window_attention_backward", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
+             v.data_ptr(), _strides(v), out.data_ptr(), lse.data_ptr(), grad.data_ptr(), _strides(grad), _DTYPES[q.dtype], b, n,
+             heads, kv_heads, dim, left, right, sinks, scale, _pointer(lengths), _pointer(visible), grad_q.data_ptr(),
+             grad_k.data_ptr(), grad_v.data_ptr(), ws.data_ptr(), ws.numel())
         need = ctx.needs_input_grad
         return grad_q if need[0] else None, grad_k if need[1] else None, grad_v if need[2] else None, None, None, None
 
@@ -295,12 +361,15 @@ def _check_scale(scale, dim):
 def _check_lengths(lengths, batch, like, like_name):
     if not torch.is_tensor(lengths):
         raise TypeError("lengths must be a torch tensor, got %s" % type(lengths).__name__)
-    if lengths.dtype != torch.int64 or tuple(lengths.shape) != (batch,):
+    if lengths.dtype != torch.int64 or lengths.shape != (batch,):
         raise ValueError("lengths must be int64 of shape (%d,), got %s %s" % (batch, lengths.dtype, tuple(lengths.shape)))
-    _cabi.same_device(like, like_name, lengths=lengths)
+    if lengths.get_device() != like.get_device():
+        _cabi.same_device(like, like_name, lengths=lengths)
 
 
 def _check_sinks(sinks):
+    if type(sinks) is int and sinks >= 0:
+        return sinks
     if sinks != int(sinks) or sinks < 0:
         raise ValueError("sinks must be a whole number, 0 or more, got %r" % (sinks,))
     return int(sinks)
@@ -319,18 +388,18 @@ def window_attention(q, k, v, window, sinks=0, *, lengths=None, visible=None, sc
     scale: of the scores, head_dim ** -0.5 if None.  Returns (batch, tokens, heads, head_dim).
 
     Differentiable with respect to q, k and v.  lengths and visible must not be changed between forward and backward."""
-    _check(q, "q")
+    _check_qkv(q, k, v)
     if q.dim() != 4:
         raise ValueError("q must have shape (batch, tokens, heads, head_dim), got %s" % (tuple(q.shape),))
     b, n, heads, dim = q.shape
     _check_dim(dim)
     for name, t in (("k", k), ("v", v)):
-        _check(t, name, q, "q")
-        if t.dim() != 4 or t.shape[:2] != q.shape[:2] or t.shape[3] != dim or t.shape[2] != k.shape[2]:
+        if t.dim() != 4 or t.shape != (b, n, k.shape[2], dim):
             raise ValueError("%s must have shape (%d, %d, kv_heads, %d) with k's heads, got %s" % (name, b, n, dim, tuple(t.shape)))
     if heads == 0 or k.shape[2] == 0 or heads % k.shape[2]:
         raise ValueError("heads (%d) must be a multiple of kv_heads (%d)" % (heads, k.shape[2]))
-    left, right = (n if w is None else w for w in window)
+    left, right = window
+    left, right = n if left is None else left, n if right is None else right
     if left != int(left) or right != int(right) or left < 0 or right < 0:
         raise ValueError("window must be two whole numbers, 0 or more, or None, got %r" % (window,))
     if lengths is not None:
@@ -339,12 +408,13 @@ def window_attention(q, k, v, window, sinks=0, *, lengths=None, visible=None, sc
     if visible is not None:
         if not torch.is_tensor(visible):
             raise TypeError("visible must be a torch tensor, got %s" % type(visible).__name__)
-        if visible.dtype != torch.bool or tuple(visible.shape) != (b, n):
+        if visible.dtype != torch.bool or visible.shape != (b, n):
             raise ValueError("visible must be bool of shape (%d, %d), got %s %s" % (b, n, visible.dtype, tuple(visible.shape)))
-        _cabi.same_device(q, "q", visible=visible)
+        if visible.get_device() != q.get_device():
+            _cabi.same_device(q, "q", visible=visible)
         visible = visible.contiguous()
     how = (min(int(left), n), min(int(right), n), min(_check_sinks(sinks), n), _check_scale(scale, dim))
-    if _cabi.needs_grad(q, k, v):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, lengths, visible, how)
     return _window_run(q, k, v, lengths, visible, how, False)[3]
 
@@ -354,6 +424,16 @@ def window_attention(q, k, v, window, sinks=0, *, lengths=None, visible=None, sc
 
 def _check_caches(k_cache, v_cache, like, kv_heads, sinks):
     batch, dim = like.shape[0], like.shape[-1]
+    try:
+        slots = k_cache.shape[1]
+        if (k_cache.dtype == v_cache.dtype == like.dtype and like.get_device() == k_cache.get_device() == v_cache.get_device()
+                and k_cache.shape == v_cache.shape == (batch, slots, kv_heads, dim) and slots > sinks and k_cache.is_contiguous()
+                and v_cache.is_contiguous()):
+            k_at, v_at = k_cache.data_ptr(), v_cache.data_ptr()
+            if k_at % 16 == 0 and v_at % 16 == 0 and abs(k_at - v_at) >= k_cache.nbytes:
+                return
+    except (AttributeError, IndexError):
+        pass
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
         _check(c, name, like, "k")
         if c.dim() != 4 or c.shape[0] != batch or c.shape[2:] != (kv_heads, dim) or c.shape != k_cache.shape:
@@ -363,8 +443,8 @@ def _check_caches(k_cache, v_cache, like, kv_heads, sinks):
             raise ValueError("%s must be contiguous and 16-byte aligned: it is written in place" % name)
     if k_cache.shape[1] <= sinks:
         raise ValueError("the caches hold %d slots: more than sinks (%d) are needed" % (k_cache.shape[1], sinks))
-    if batch and k_cache.data_ptr() == v_cache.data_ptr():
-        raise ValueError("k_cache and v_cache must be two tensors")
+    if batch:
+        raise ValueError("k_cache and v_cache must be two tensors that do not overlap")
 
 
 def _written(*tensors):
@@ -380,10 +460,9 @@ def window_cache_fill(k, v, k_cache, v_cache, lengths, sinks=0):
     (batch,) int64.  Token t goes to slot t if t < sinks, else to slot sinks + (t - sinks) % window; of each sequence the first
     `sinks` and the last `window` tokens are stored and slots that no token belongs to stay as they are.  The same `lengths`
     (at most `tokens` each) is what the next window_attention_step takes.  Forward only."""
-    _check(k, "k")
+    _check_qkv(k, k, v)
     if k.dim() != 4:
         raise ValueError("k must have shape (batch, tokens, kv_heads, head_dim), got %s" % (tuple(k.shape),))
-    _check(v, "v", k, "k")
     if v.shape != k.shape:
         raise ValueError("v must have k's shape %s, got %s" % (tuple(k.shape), tuple(v.shape)))
     b, n, kv_heads, dim = k.shape
@@ -391,11 +470,12 @@ def window_cache_fill(k, v, k_cache, v_cache, lengths, sinks=0):
     sinks = _check_sinks(sinks)
     _check_caches(k_cache, v_cache, k, kv_heads, sinks)
     _check_lengths(lengths, b, k, "k")
-    _cabi.forward_only("window_cache_fill", k, v, k_cache, v_cache)
+    if torch.is_grad_enabled():
+        _cabi.forward_only("window_cache_fill", k, v, k_cache, v_cache)
     k, v, lengths = _tokens(k), _tokens(v), lengths.contiguous()
-    _run(k.device, "mvx_window_cache_fill", _cabi.load().mvx_window_cache_fill, k.data_ptr(), _strides(k), v.data_ptr(),
-         _strides(v), _DTYPES[k.dtype], lengths.data_ptr(), b, n, kv_heads, dim, k_cache.shape[1] - sinks, sinks,
-         k_cache.data_ptr(), v_cache.data_ptr())
+    _run(k.get_device(), "window_cache_fill", "mvx_window_cache_fill", k.data_ptr(), _strides(k), v.data_ptr(), _strides(v),
+         _DTYPES[k.dtype], lengths.data_ptr(), b, n, kv_heads, dim, k_cache.shape[1] - sinks, sinks, k_cache.data_ptr(),
+         v_cache.data_ptr())
     _written(k_cache, v_cache)
 
 
@@ -408,14 +488,13 @@ def window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks=0, *, scale=
     (batch, heads, head_dim): the row that window_attention gives the token with window (window - 1, 0).  A negative length
     marks an idle stream: its slots and length stay as they are and its row is zero.  Two calls on the same ring must not
     overlap.  Forward only."""
-    _check(q, "q")
+    _check_qkv(q, k, v)
     if q.dim() != 3:
         raise ValueError("q must have shape (batch, heads, head_dim), got %s" % (tuple(q.shape),))
     b, heads, dim = q.shape
     _check_dim(dim)
     for name, t in (("k", k), ("v", v)):
-        _check(t, name, q, "q")
-        if t.dim() != 3 or t.shape[0] != b or t.shape[2] != dim or t.shape[1] != k.shape[1]:
+        if t.dim() != 3 or t.shape != (b, k.shape[1], dim):
             raise ValueError("%s must have shape (%d, kv_heads, %d) with k's heads, got %s" % (name, b, dim, tuple(t.shape)))
     kv_heads = k.shape[1]
     if heads == 0 or kv_heads == 0 or heads % kv_heads:
@@ -425,17 +504,18 @@ def window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks=0, *, scale=
     _check_lengths(lengths, b, q, "q")
     if not lengths.is_contiguous():
         raise ValueError("lengths must be contiguous: it is written in place")
-    _cabi.forward_only("window_attention_step", q, k, v, k_cache, v_cache)
+    if torch.is_grad_enabled():
+        _cabi.forward_only("window_attention_step", q, k, v, k_cache, v_cache)
     scale = _check_scale(scale, dim)
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     window = k_cache.shape[1] - sinks
-    lib = _cabi.load()
     out = torch.empty((b, heads, dim), dtype=q.dtype, device=q.device)
-    ws = _workspace(lib.mvx_window_attention_step_workspace_bytes(b, heads, kv_heads, dim, window, sinks), q.device)
-    _run(q.device, "mvx_window_attention_step", lib.mvx_window_attention_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-         _DTYPES[q.dtype], b, heads, kv_heads, dim, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(),
-         lengths.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel())
+    n_bytes = _cabi.load().mvx_window_attention_step_workspace_bytes(b, heads, kv_heads, dim, window, sinks)
+    ws = _workspace(n_bytes, q.device) if n_bytes else None
+    _run(q.get_device(), "window_attention_step", "mvx_window_attention_step", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+         _DTYPES[q.dtype], b, heads, kv_heads, dim, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
+         out.data_ptr(), _pointer(ws), n_bytes)
     _written(k_cache, v_cache, lengths)
     return out
