@@ -3,10 +3,10 @@
 //   key j is seen by query i iff j <= i + right and (j >= i - left or j < sinks), j < length, visible[j]
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i) over the seen keys; a row that sees none is zero
 //
-// One workgroup of 4 waves takes 128 queries of one head, 32 per wave, and walks the tiles of 64 keys that any of them
-// sees: first those of the sinks, then the window.  Scores come out transposed (keys in registers, queries in lanes), so the
+// A wave takes 32 queries of one head; a workgroup of 4 waves (or of one, for short windows) walks the tiles of 64 (32) keys
+// that any of its queries sees: first those of the sinks, then the window.  Scores come out transposed (keys in registers, queries in lanes), so the
 // softmax of a query runs inside a lane and its partner 32 lanes on, with a running maximum and sum, and the weighted sum of
-// the values takes the scores where they lie.  A tile is held in LDS for all four waves and the next one travels from memory
+// the values takes the scores where they lie.  A tile is held in LDS for all waves and the next one travels from memory
 // meanwhile; tiles that every query sees whole skip the mask, and a wave skips a tile that none of its queries sees.
 // Scores and sums are float32; the weights (at most 1) are rounded to the element type for the second product, the sum that
 // divides the result is taken before that rounding.
@@ -16,15 +16,15 @@ namespace mvx {
 
 namespace {
 
-constexpr int kWaves = 4, kBQ = 32 * kWaves, kBK = 64;
+constexpr int key_step(int waves) { return waves == 1 ? 32 : 64; }  // keys of a tile
 constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2^15
 
 // The registers are cut for two waves per SIMD where they suffice: with one, a long prompt of heads of 128 took 1.8 times as long.
-template <typename T, int DP>
+template <typename T, int DP, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
     TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
     using Tl = Tiles<T, DP>;
-    constexpr int DT = DP / 32;
+    constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = key_step(kWaves);
     __shared__ __attribute__((aligned(16))) T k_tile[2][kBK * Tl::LD];
     __shared__ __attribute__((aligned(16))) T v_tile[2][kBK * Tl::LD];
     // heads that share keys, then blocks of queries, are neighbours on one XCD
@@ -215,24 +215,28 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &kt)) != MVX_OK) return rc;
     if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && aligned16(out), MVX_ERR_INVALID_ARGUMENT, "%s: out is null or not 16-byte aligned", name);
-    const int q_blocks = static_cast<int>((n_tokens + kBQ - 1) / kBQ);
+    // Four waves share their tiles, and wait for each other's: of a window of w keys a wave sees 32 + w, the workgroup 128 + w.
+    // Short windows are therefore walked by single waves (257 tokens x 4 heads x 64 float32, 33 keys: 19.0 -> 11.9 us; 2000 x 16
+    // x 32, 127 keys: 15.5 -> 12.3; from 255 keys on, and with heads above 64, four waves are as fast or faster).
+    const int waves = dim <= 64 && static_cast<int64_t>(s.left) + s.right < 128 ? 1 : 4;
+    const int q_blocks = static_cast<int>((n_tokens + 32 * waves - 1) / (32 * waves));
     MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
                 name);
     const unsigned blocks = static_cast<unsigned>(n_seqs * heads * q_blocks);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
-        const auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
-                               static_cast<T*>(out), lse);
+        const auto launch = [&](auto alone, auto four) {
+            hipLaunchKernelGGL(waves == 1 ? alone : four, dim3(blocks), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), qt, kt,
+                               vt, s, q_blocks, static_cast<T*>(out), lse);
         };
         if (dim <= 32)
-            launch(window_attention<T, 32>);
+            launch(window_attention<T, 32, 1>, window_attention<T, 32, 4>);
         else if (dim <= 64)
-            launch(window_attention<T, 64>);
+            launch(window_attention<T, 64, 1>, window_attention<T, 64, 4>);
         else if (dim <= 96)
-            launch(window_attention<T, 96>);
+            launch(window_attention<T, 96, 1>, window_attention<T, 96, 4>);
         else
-            launch(window_attention<T, 128>);
+            launch(window_attention<T, 128, 1>, window_attention<T, 128, 4>);
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });
