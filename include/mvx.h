@@ -442,9 +442,11 @@ int mvx_window_attention_backward(const void* q, const int64_t* q_strides, const
  * q            [n_seqs][heads][dim] of dtype; k, v [n_seqs][kv_heads][dim]; contiguous
  * k_cache, v_cache  [n_seqs][sinks + window][kv_heads][dim], read and written;  lengths [n_seqs], read and written
  * out          [n_seqs][heads][dim]
- * workspace    mvx_window_attention_step_workspace_bytes() bytes, 4-byte aligned; q, caches: 16-byte aligned
+ * workspace    mvx_window_attention_step_workspace_bytes() bytes (0 for short rings: NULL); q, caches and workspace 16-byte
+ *              aligned
  */
-size_t mvx_window_attention_step_workspace_bytes(int64_t n_seqs, int heads, int kv_heads, int dim, int64_t window, int64_t sinks);
+size_t mvx_window_attention_step_workspace_bytes(int dtype, int64_t n_seqs, int heads, int kv_heads, int dim, int64_t window,
+                                                 int64_t sinks);
 int mvx_window_attention_step(const void* q, const void* k, const void* v, int dtype, int64_t n_seqs, int heads, int kv_heads,
                               int dim, int64_t window, int64_t sinks, float scale, void* k_cache, void* v_cache,
                               int64_t* lengths, void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -69,7 +69,7 @@ SIGNATURES = {
     "mvx_window_attention_backward_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int, _i64, _i64]),
     "mvx_window_attention_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _int, _int,
                                              _int, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "mvx_window_attention_step_workspace_bytes": (_sz, [_i64, _int, _int, _int, _i64, _i64]),
+    "mvx_window_attention_step_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int, _i64, _i64]),
     "mvx_window_attention_step": (_int, [_vp, _vp, _vp, _int, _i64, _int, _int, _int, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp,
                                          _sz, _vp]),
     "mvx_window_cache_fill": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _int, _int, _i64, _i64, _vp, _vp, _vp]),

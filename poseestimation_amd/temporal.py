@@ -512,7 +512,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks=0, *, scale=
         q = q.clone()
     window = k_cache.shape[1] - sinks
     out = torch.empty((b, heads, dim), dtype=q.dtype, device=q.device)
-    n_bytes = _cabi.load().mvx_window_attention_step_workspace_bytes(b, heads, kv_heads, dim, window, sinks)
+    n_bytes = _cabi.load().mvx_window_attention_step_workspace_bytes(_DTYPES[q.dtype], b, heads, kv_heads, dim, window, sinks)
     ws = _workspace(n_bytes, q.device) if n_bytes else None
     _run(q.get_device(), "window_attention_step", "mvx_window_attention_step", q.data_ptr(), k.data_ptr(), v.data_ptr(),
          _DTYPES[q.dtype], b, heads, kv_heads, dim, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),

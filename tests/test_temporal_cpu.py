@@ -99,7 +99,7 @@ def test_ring_argument_checks():
     assert step(q=None) == BAD and step(cache=None) == BAD and step(cache=SOME + 8) == BAD and step(dtype=3) == BAD
     assert step(window=0) == BAD and step(sinks=-1) == BAD and step(heads=3) == BAD and step(dim=20) == BAD and step(scale=-1.0) == BAD
     assert step(dim=256) == UNSUPPORTED and step(seqs=70000) == UNSUPPORTED
-    assert step(ws=3) == _cabi.MVX_ERR_WORKSPACE
+    assert step(ws=3, window=1 << 20) == _cabi.MVX_ERR_WORKSPACE
     st = S3(4 * 2 * 16, 2 * 16, 16)
 
     def fill(k=SOME, strides=st, tokens=4, window=8, sinks=1, cache=SOME):
