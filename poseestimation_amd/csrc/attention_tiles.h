@@ -6,8 +6,8 @@
 //   cols_times:  A[d][col]    += sum_row tile[row][d] * S[row][col] (S as rows_times left it)
 // rows_times leaves register i of a lane at row 8 (i / 4) + 4 half + i % 4.  The second product sums over rows, whose order
 // is free as long as both operands agree, so it takes the registers as they lie: its other operand is read from the same
-// row-major tile, for 16-bit types by the transposing LDS read (4 rows x 16 columns per 16 lanes), for float32 one row per
-// instruction.  Nothing is shuffled between lanes and no tile is stored twice.
+// row-major tile by the transposing LDS read (4 rows x 16 columns per 16 lanes).  Nothing is shuffled between lanes and no tile
+// is stored twice.
 #pragma once
 
 #include "element.h"
@@ -63,6 +63,7 @@ struct Tiles;
 template <typename T, int DP>
 struct Tiles16 {
     typedef typename Element<T>::vec_t v8;
+    typedef T Cell;  // what a tile holds
     static constexpr int VEC = 8;
     static constexpr int STEPS = DP / 16;
     // Tiles of 32, 64 and 128 columns are stored without padding; 16-byte chunk c of row r lies at chunk c ^ twist(r).  The
@@ -94,14 +95,6 @@ struct Tiles16 {
             f.step[s] = valid && d < dim ? *reinterpret_cast<const v8*>(row + d) : v8{};
         }
     }
-    static __device__ __forceinline__ float dot(const Frag& a, const Frag& b) {  // this half's share
-        float r = 0.0f;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r = fmaf(static_cast<float>(a.step[s][e]), static_cast<float>(b.step[s][e]), r);
-        return r;
-    }
     static __device__ __forceinline__ v16f mfma(v8 a, v8 b, v16f c) {
         if constexpr (__is_same(T, bf16))
             return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -114,18 +107,22 @@ struct Tiles16 {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) p.a[s] = *reinterpret_cast<const v8*>(tile + at(r, 16 * s + 8 * half));
     }
-    static __device__ __forceinline__ void cols(Pool& p, const T* tile) {
+    // two transposing reads: 4 values each from 4 rows
+    static __device__ __forceinline__ v8 turned(const T* lower, const T* upper) {
         typedef __attribute__((address_space(3))) v4s lds_v4s;
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(lower));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(upper));
+        const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(v8, both);
+    }
+    static __device__ __forceinline__ void cols(Pool& p, const T* tile) {
         const int l = lane_id(), j = l & 15, r = 4 * (l >> 5) + (j >> 2), c = 16 * ((l >> 4) & 1) + 4 * (j & 3);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) {
                 // bit 2 of c selects the half of a chunk and is not twisted
-                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + at(16 * s + r, 32 * dt + c)));
-                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + at(16 * s + r + 8, 32 * dt + c)));
-                const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                p.a[s * (DP / 32) + dt] = __builtin_bit_cast(v8, both);
+                p.a[s * (DP / 32) + dt] = turned(tile + at(16 * s + r, 32 * dt + c), tile + at(16 * s + r + 8, 32 * dt + c));
             }
     }
     static __device__ __forceinline__ v16f rows_times(const Pool& p, const Frag& f) {
@@ -150,67 +147,120 @@ struct Tiles<bf16, DP> : Tiles16<bf16, DP> {};
 template <int DP>
 struct Tiles<f16, DP> : Tiles16<f16, DP> {};
 
+// float32 on the bfloat16 matrix units, which are sixteen times as fast as the float32 ones: a value is the sum of three
+// bfloat16 parts, x = a + b + c, each the rounding of what the parts before it leave (8 bits of significand each, together all
+// 24), and a product of two values is the sum of the six products of parts that matter,
+//
+//   x y = a a' + (a b' + b a') + (a c' + b b' + c a'),
+//
+// added smallest first in the float32 accumulators.  |b| <= 2^-9 |x| and |c| <= 2^-18 |x| (1 + 2^-9), so the three products left
+// out are below 2^-26 |x y| together: less than the rounding of one float32 product.  A value that is not finite has parts that
+// are NaN; columns that see one are computed again pair by pair.  Tiles hold the three parts of a row one behind the other.
 template <int DP>
 struct Tiles<float, DP> {
+    typedef Tiles16<bf16, DP> Part;
+    typedef typename Part::v8 v8;
+    typedef bf16 Cell;
     static constexpr int VEC = 4;
-    static constexpr int STEPS = DP / 8;
-    static constexpr int LD = DP + 4;
-    static __device__ __forceinline__ int at(int r, int col) { return r * LD + col; }
+    static constexpr int STEPS = Part::STEPS;
+    static constexpr int LD = 3 * Part::LD;
+    static __device__ __forceinline__ int at(int r, int col) { return r * LD + (col ^ (Part::twist(r) << 3)); }
     struct Frag {
-        v4f step[STEPS];  // d = 8 t + 4 half + e: the order the row reads of 16 bytes give
+        v8 step[3][STEPS];
     };
-    struct Pool {
-        v4f a[STEPS];
+    struct Pool {  // three parts are too many registers to fill ahead of their use
+        const Cell* tile;
     };
+    static __device__ __forceinline__ void split(float x, bf16& a, bf16& b, bf16& c) {
+        a = static_cast<bf16>(x);
+        const float rest = x - static_cast<float>(a);
+        b = static_cast<bf16>(rest);
+        c = static_cast<bf16>(rest - static_cast<float>(b));
+    }
     static __device__ __forceinline__ void load_column(Frag& f, const float* row, int dim, bool valid) {
         const int half = lane_id() >> 5;
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-            const int d = 8 * t + 4 * half;
-            f.step[t] = valid && d < dim ? *reinterpret_cast<const v4f*>(row + d) : v4f{};
+        for (int s = 0; s < STEPS; ++s) {
+            const int d = 16 * s + 8 * half;
+            const bool there = valid && d < dim;
+            const v4f lo = there ? *reinterpret_cast<const v4f*>(row + d) : v4f{}, hi = there ? *reinterpret_cast<const v4f*>(row + d + 4) : v4f{};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bf16 a, b, c;
+                split(e < 4 ? lo[e % 4] : hi[e % 4], a, b, c);
+                f.step[0][s][e] = a, f.step[1][s][e] = b, f.step[2][s][e] = c;
+            }
         }
     }
-    static __device__ __forceinline__ float dot(const Frag& a, const Frag& b) {
-        float r = 0.0f;
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r = fmaf(a.step[t][e], b.step[t][e], r);
-        return r;
-    }
-    static __device__ __forceinline__ void rows(Pool& p, const float* tile) {
-        const float* q = tile + (lane_id() & 31) * LD + 4 * (lane_id() >> 5);
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) p.a[t] = *reinterpret_cast<const v4f*>(q + 8 * t);
-    }
-    static __device__ __forceinline__ void cols(Pool& p, const float* tile) {
-        const float* q = tile + 4 * (lane_id() >> 5) * LD + (lane_id() & 31);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) {
-                const int n = i * (DP / 32) + dt;
-                p.a[n / 4][n % 4] = q[(8 * (i / 4) + i % 4) * LD + 32 * dt];
-            }
+    static __device__ __forceinline__ void rows(Pool& p, const Cell* tile) { p.tile = tile; }
+    static __device__ __forceinline__ void cols(Pool& p, const Cell* tile) { p.tile = tile; }
+    static __device__ __forceinline__ v16f six(const v8 (&x)[3], const v8 (&y)[3], v16f acc) {
+        acc = Part::mfma(x[0], y[2], acc);
+        acc = Part::mfma(x[2], y[0], acc);
+        acc = Part::mfma(x[1], y[1], acc);
+        acc = Part::mfma(x[0], y[1], acc);
+        acc = Part::mfma(x[1], y[0], acc);
+        return Part::mfma(x[0], y[0], acc);
     }
     static __device__ __forceinline__ v16f rows_times(const Pool& p, const Frag& f) {
+        const int r = lane_id() & 31, half = lane_id() >> 5;
         v16f acc = {};
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t)
+        for (int s = 0; s < STEPS; ++s) {
+            v8 x[3], y[3];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(p.a[t][e], f.step[t][e], acc, 0, 0, 0);
+            for (int n = 0; n < 3; ++n) {
+                x[n] = *reinterpret_cast<const v8*>(p.tile + n * Part::LD + at(r, 16 * s + 8 * half));
+                y[n] = f.step[n][s];
+            }
+            acc = six(x, y, acc);
+        }
         return acc;
     }
     static __device__ __forceinline__ void cols_times(const Pool& p, const v16f& w, v16f (&acc)[DP / 32]) {
+        const int l = lane_id(), j = l & 15, r = 4 * (l >> 5) + (j >> 2), col = 16 * ((l >> 4) & 1) + 4 * (j & 3);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int s = 0; s < 2; ++s) {
+            v8 y[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bf16 a, b, c;
+                split(w[8 * s + e], a, b, c);
+                y[0][e] = a, y[1][e] = b, y[2][e] = c;
+            }
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) {
-                const int n = i * (DP / 32) + dt;
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(p.a[n / 4][n % 4], w[i], acc[dt], 0, 0, 0);
+                v8 x[3];
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    x[n] = Part::turned(p.tile + n * Part::LD + at(16 * s + r, 32 * dt + col),
+                                        p.tile + n * Part::LD + at(16 * s + r + 8, 32 * dt + col));
+                acc[dt] = six(x, y, acc[dt]);
             }
+        }
     }
 };
+
+// Keys (or queries) of a tile that a workgroup shares.
+template <typename T>
+constexpr int kTileRows = sizeof(T) == 4 ? 32 : 64;
+
+// This half's share of the product of two rows, in the columns that load_column gives it.
+template <typename T>
+__device__ __forceinline__ float half_dot(const T* a, const T* b, int dim, bool valid) {
+    float r = 0.0f;
+    if (valid)
+        for (int d = 8 * (lane_id() >> 5); d < dim; d += 16)
+#pragma unroll
+            for (int e = 0; e < 8; e += Element<T>::vec) {
+                float x[Element<T>::vec], y[Element<T>::vec];
+                load_vec<T>(a + d + e, x);
+                load_vec<T>(b + d + e, y);
+#pragma unroll
+                for (int i = 0; i < Element<T>::vec; ++i) r = fmaf(x[i], y[i], r);
+            }
+    return r;
+}
 
 // ROWS x DP tile on its way from global memory to LDS, carried by THREADS neighbouring threads (the workgroup, or a wave): held
 // in registers while the previous tile is worked on.
@@ -240,12 +290,26 @@ struct TileInFlight {
         for (int n = 0; n < N; ++n)
             v[n] = __builtin_bit_cast(typename Element<T>::vec_t, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[n], 0, 0));
     }
-    __device__ __forceinline__ void store(T* tile) const {
+    __device__ __forceinline__ void store(typename Tiles<T, DP>::Cell* tile) const {
+        using Tl = Tiles<T, DP>;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = threadIdx.x % THREADS + n * THREADS, r = i / PER_ROW, c = i % PER_ROW * VEC;
-            if (ALL % THREADS == 0 || i < ALL)
-                *reinterpret_cast<typename Element<T>::vec_t*>(tile + Tiles<T, DP>::at(r, c)) = v[n];
+            if (ALL % THREADS != 0 && i >= ALL) continue;
+            if constexpr (sizeof(T) == 4) {
+                typedef bf16 v4b __attribute__((ext_vector_type(4)));
+                v4b part[3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bf16 x, y, z;
+                    Tl::split(v[n][e], x, y, z);
+                    part[0][e] = x, part[1][e] = y, part[2][e] = z;
+                }
+#pragma unroll
+                for (int m = 0; m < 3; ++m) *reinterpret_cast<v4b*>(tile + m * Tl::Part::LD + Tl::at(r, c)) = part[m];
+            } else {
+                *reinterpret_cast<typename Element<T>::vec_t*>(tile + Tl::at(r, c)) = v[n];
+            }
         }
     }
     // zeros in the rows whose bit is clear in `keep`: what a hidden token holds never enters a product

@@ -16,17 +16,16 @@ namespace mvx {
 
 namespace {
 
-constexpr int key_step(int waves) { return waves == 1 ? 32 : 64; }  // keys of a tile
 constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2^15
 
 // The registers are cut for two waves per SIMD where they suffice: with one, a long prompt of heads of 128 took 1.8 times as long.
 template <typename T, int DP, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
+__global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
     TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
     using Tl = Tiles<T, DP>;
-    constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = key_step(kWaves);
-    __shared__ __attribute__((aligned(16))) T k_tile[2][kBK * Tl::LD];
-    __shared__ __attribute__((aligned(16))) T v_tile[2][kBK * Tl::LD];
+    constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = kWaves == 1 ? 32 : kTileRows<T>;  // queries of the workgroup, keys of a tile
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kBK * Tl::LD];
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kBK * Tl::LD];
     // heads that share keys, then blocks of queries, are neighbours on one XCD
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int share = a.heads / a.kv_heads;
@@ -86,7 +85,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= 256 ? 2 : 1) void wi
         if (t + 1 < tiles.count) keep_next = put(t + 1);
         if (t + 2 < tiles.count) fetch(t + 2);
         const int k0 = tiles.key0(t, kBK);
-        const T *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+        const typename Tl::Cell *kt = k_tile[t & 1], *vt = v_tile[t & 1];
 #pragma unroll 1  // two copies need more registers than two waves per SIMD have
         for (int b = 0; b < kBK; b += 32) {
             if (!sees_any(a, w0, k0 + b, 32, length)) continue;
@@ -216,27 +215,31 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && aligned16(out), MVX_ERR_INVALID_ARGUMENT, "%s: out is null or not 16-byte aligned", name);
     // Four waves share their tiles, and wait for each other's: of a window of w keys a wave sees 32 + w, the workgroup 128 + w.
-    // Short windows are therefore walked by single waves (257 tokens x 4 heads x 64 float32, 33 keys: 19.0 -> 11.9 us; 2000 x 16
-    // x 32, 127 keys: 15.5 -> 12.3; from 255 keys on, and with heads above 64, four waves are as fast or faster).
-    const int waves = dim <= 64 && static_cast<int64_t>(s.left) + s.right < 128 ? 1 : 4;
+    // Short windows are therefore walked by single waves where their tiles leave room for enough of them: always with 16-bit
+    // types (4 x 4096 tokens x 8 heads x 64, 33 keys: 22.8 -> 20.7 us; from 255 keys on four waves are faster), with float32, whose
+    // tiles are three times as large, up to one round of them (257 tokens x 4 heads x 64, 33 keys: 15.9 -> 12.7 us; 4 x 2000 x 4 x
+    // 32, 127 keys: 14.9 -> 12.8, but 4 x 4096 x 8 x 32, 33 keys: 27.4 -> 31.8).
+    const int64_t all_waves = n_seqs * heads * ((n_tokens + 31) / 32);
+    const bool room = dtype != MVX_F32 || all_waves <= (dim <= 32 ? 1536 : 768);
+    const int waves = dim <= 64 && static_cast<int64_t>(s.left) + s.right < 128 && room ? 1 : 4;
     const int q_blocks = static_cast<int>((n_tokens + 32 * waves - 1) / (32 * waves));
     MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
                 name);
     const unsigned blocks = static_cast<unsigned>(n_seqs * heads * q_blocks);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
-        const auto launch = [&](auto alone, auto four) {
-            hipLaunchKernelGGL(waves == 1 ? alone : four, dim3(blocks), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), qt, kt,
-                               vt, s, q_blocks, static_cast<T*>(out), lse);
+        const auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
+                               static_cast<T*>(out), lse);
         };
         if (dim <= 32)
-            launch(window_attention<T, 32, 1>, window_attention<T, 32, 4>);
+            waves == 1 ? launch(window_attention<T, 32, 1>) : launch(window_attention<T, 32, 4>);
         else if (dim <= 64)
-            launch(window_attention<T, 64, 1>, window_attention<T, 64, 4>);
+            waves == 1 ? launch(window_attention<T, 64, 1>) : launch(window_attention<T, 64, 4>);
         else if (dim <= 96)
-            launch(window_attention<T, 96, 1>, window_attention<T, 96, 4>);
+            launch(window_attention<T, 96, 4>);
         else
-            launch(window_attention<T, 128, 1>, window_attention<T, 128, 4>);
+            launch(window_attention<T, 128, 4>);
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });

@@ -17,7 +17,7 @@ namespace mvx {
 
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlock = 32 * kWaves, kTile = 64;
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlock = 32 * kWaves;
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
@@ -25,8 +25,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
                                                                 T* __restrict__ dq) {
     using Tl = Tiles<T, DP>;
-    __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * Tl::LD];
-    __shared__ __attribute__((aligned(16))) T v_tile[2][kTile * Tl::LD];
+    constexpr int kTile = kTileRows<T>;
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kTile * Tl::LD];
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int share = a.heads / a.kv_heads;
     const int in_group = id % share;
@@ -46,13 +47,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     typename Tl::Frag qf, gf;
     Tl::load_column(qf, static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head, a.dim, live);
     Tl::load_column(gf, static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head, a.dim, live);
-    float my_delta, my_lse = 0.0f;
-    {
-        typename Tl::Frag of;
-        Tl::load_column(of, static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head, a.dim,
-                        live);
-        my_delta = both_halves_sum(Tl::dot(gf, of));
-    }
+    float my_lse = 0.0f;
+    const float my_delta = both_halves_sum(half_dot(static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head,
+                                        static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head,
+                                        a.dim, live));
     const int64_t at_row = (seq * a.heads + head) * a.n_tokens + mine;
     if (live) my_lse = lse[at_row];
     if (mine < a.n_tokens && half == 0) delta[at_row] = my_delta;
@@ -95,7 +93,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
         if (t + 1 < tiles.count) keep_next = put(t + 1);
         if (t + 2 < tiles.count) fetch(t + 2);
         const int k0 = tiles.key0(t, kTile);
-        const T *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+        const typename Tl::Cell *kt = k_tile[t & 1], *vt = v_tile[t & 1];
         const int at = k0 + 4 * half;
         const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
         const uint64_t bits = keep >> (4 * half);
@@ -150,18 +148,21 @@ __device__ __forceinline__ int64_t sink_sums(const AttentionShape& a, int64_t se
 // One chunk of the queries behind the window of 32 sinks.  Every wave takes 32 queries of one head at a time through tiles of
 // its own (no barrier in the loop); the waves' sums are added in order at the end.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
+constexpr int kSinkWaves = sizeof(T) * DP > 384 ? 2 : 4;  // float32 heads of 128: 49 KB of tiles per wave
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sinks(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
                                                                    AttentionShape a, int chunk, int chunks,
                                                                    const float* __restrict__ lse, const float* __restrict__ delta,
                                                                    float* __restrict__ partial) {
     using Tl = Tiles<T, DP>;
+    constexpr int kOwn = kSinkWaves<T, DP>;
     struct WaveTiles {
-        __attribute__((aligned(16))) T q[32 * Tl::LD];
-        __attribute__((aligned(16))) T g[32 * Tl::LD];
+        __attribute__((aligned(16))) typename Tl::Cell q[32 * Tl::LD];
+        __attribute__((aligned(16))) typename Tl::Cell g[32 * Tl::LD];
         __attribute__((aligned(16))) float stats[2][32];  // lse, delta
     };
     __shared__ union Shared {
-        WaveTiles wave[kWaves];
+        WaveTiles wave[kOwn];
         float sums[kSinkSums<DP>];
     } shared;
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
     const int share = a.heads / a.kv_heads;
     const int lane = lane_id(), half = lane >> 5, wave = wave_id();
     const int length = seq_length(a, seq), mine = block * 32 + (lane & 31);
-    const int begin = window_end(a, block / kWaves * kBlock, length) + c * chunk, end = min(length, begin + chunk);
+    const int begin = window_end(a, block * 32 / kBlock * kBlock, length) + c * chunk, end = min(length, begin + chunk);
     if (begin >= end) return;  // the block of keys reads the chunks that its length leaves, no others
     const int per_head = (end - begin + 31) / 32, items = per_head * share;
 
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
     TileInFlight<T, DP, 32, 64> q_next, g_next;
     q_next.place(q.token, a.dim);
     g_next.place(g.token, a.dim);
-    for (int t = wave; t < items; t += kWaves) {
+    for (int t = wave; t < items; t += kOwn) {
         const int head = kv_head * share + t / per_head, i0 = begin + t % per_head * 32;
         q_next.load(static_cast<const T*>(q.p) + seq * q.seq + head * q.head, q.token, i0, end);
         g_next.load(static_cast<const T*>(g.p) + seq * g.seq + head * g.head, g.token, i0, end);
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
         Tl::cols_times(more, dp, dk_acc);
     }
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kOwn; ++w) {
         if (w == wave) {
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(kThreads) void window_attention_sinks(TokenTensor q
         __syncthreads();
     }
     float* out = partial + sink_sums<DP>(a, seq, kv_head, block, chunks) + c * kSinkSums<DP>;
-    for (int i = threadIdx.x; i < kSinkSums<DP>; i += kThreads) out[i] = shared.sums[i];
+    for (int i = threadIdx.x; i < kSinkSums<DP>; i += 64 * kOwn) out[i] = shared.sums[i];
 }
 
 // Keys [k0, k0 + 128) of one key/value head: the queries of the block's window, then the sums that window_attention_sinks
@@ -252,8 +253,9 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
                                                                  const float* __restrict__ delta, const float* __restrict__ partial,
                                                                  T* __restrict__ dk, T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
-    __shared__ __attribute__((aligned(16))) T q_tile[2][kTile * Tl::LD];
-    __shared__ __attribute__((aligned(16))) T g_tile[2][kTile * Tl::LD];
+    constexpr int kTile = kTileRows<T>;
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell q_tile[2][kTile * Tl::LD];
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell g_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse, delta
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int block = id % k_blocks;
@@ -309,7 +311,7 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
         if (t + 1 < tiles) put(t + 1);
         if (t + 2 < tiles) fetch(t + 2);
         if (w0 >= length) continue;
-        const T *qt = q_tile[t & 1], *gt = g_tile[t & 1];
+        const typename Tl::Cell *qt = q_tile[t & 1], *gt = g_tile[t & 1];
         const int at = i0 + 4 * half, lo_r = lo - at, hi_r = min(hi, end - 1) - at;
 #pragma unroll 1  // two copies need more registers than two waves per SIMD have
         for (int b = 0; b < kTile / 32; ++b) {
@@ -457,25 +459,25 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
-        const auto launch = [&](auto dq_kernel, auto sinks_kernel, auto dkv_kernel) {
+        const auto launch = [&](auto dq_kernel, auto sinks_kernel, int sink_waves, auto dkv_kernel) {
             const float* d = delta;
             hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * blocks)), dim3(kThreads), 0, st, qt, kt, vt,
                                ot, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
             if (f.chunks > 0)
                 hipLaunchKernelGGL(sinks_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks * f.chunks)),
-                                   dim3(kThreads), 0, st, qt, kt, vt, gt, s, f.chunk, f.chunks, lse, d, partial);
+                                   dim3(64 * sink_waves), 0, st, qt, kt, vt, gt, s, f.chunk, f.chunks, lse, d, partial);
             hipLaunchKernelGGL(dkv_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
                                vt, gt, s, scale, blocks, f.chunk, f.chunks, lse, d, static_cast<const float*>(partial),
                                static_cast<T*>(grad_k), static_cast<T*>(grad_v));
         };
         if (dim <= 32)
-            launch(window_attention_dq<T, 32>, window_attention_sinks<T, 32>, window_attention_dkv<T, 32>);
+            launch(window_attention_dq<T, 32>, window_attention_sinks<T, 32>, kSinkWaves<T, 32>, window_attention_dkv<T, 32>);
         else if (dim <= 64)
-            launch(window_attention_dq<T, 64>, window_attention_sinks<T, 64>, window_attention_dkv<T, 64>);
+            launch(window_attention_dq<T, 64>, window_attention_sinks<T, 64>, kSinkWaves<T, 64>, window_attention_dkv<T, 64>);
         else if (dim <= 96)
-            launch(window_attention_dq<T, 96>, window_attention_sinks<T, 96>, window_attention_dkv<T, 96>);
+            launch(window_attention_dq<T, 96>, window_attention_sinks<T, 96>, kSinkWaves<T, 96>, window_attention_dkv<T, 96>);
         else
-            launch(window_attention_dq<T, 128>, window_attention_sinks<T, 128>, window_attention_dkv<T, 128>);
+            launch(window_attention_dq<T, 128>, window_attention_sinks<T, 128>, kSinkWaves<T, 128>, window_attention_dkv<T, 128>);
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });
