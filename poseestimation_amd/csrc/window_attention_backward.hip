@@ -9,7 +9,7 @@
 //   2. keys in lanes, walking the tiles of queries that see them, over all heads that share the keys: dk and dv.
 // In the second a block of sink keys is seen by the whole rest of the sequence.  The queries behind the block's own window
 // are therefore cut into chunks that a third kernel takes, between the two: a workgroup per chunk and 32 sinks, its waves
-// on queries of their own, its sum left in float32; the block of keys adds its chunks' sums in order.
+// on queries of their own, its sum left in float32.  A fourth adds the chunks in order, and the block of keys starts from that.
 // p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.
 #include "attention_tiles.h"
 
@@ -137,9 +137,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
 __device__ __forceinline__ int window_end(const AttentionShape& a, int k0, int length) {
     return min(length, k0 + kBlock + a.left);
 }
-// Sums of 32 sinks over one chunk of queries, in the registers' order: [register][dk, dv][lane].
+// Sums of 32 sinks over one chunk of queries, in the order of the registers: [4 registers][dk, dv][lane][4].
 template <int DP>
 constexpr int64_t kSinkSums = static_cast<int64_t>(DP) * 32 * 2;
+template <int DP>
+__device__ __forceinline__ v4f* sink_vec(float* sums, int dt, int i4, int which) {
+    return reinterpret_cast<v4f*>(sums) + ((dt * 4 + i4) * 2 + which) * 64 + lane_id();
+}
 template <int DP>
 __device__ __forceinline__ int64_t sink_sums(const AttentionShape& a, int64_t seq, int kv_head, int sink_block, int chunks) {
     return ((seq * a.kv_heads + kv_head) * ((a.sinks + 31) / 32) + sink_block) * chunks * kSinkSums<DP>;
@@ -150,7 +154,7 @@ __device__ __forceinline__ int64_t sink_sums(const AttentionShape& a, int64_t se
 template <typename T, int DP>
 constexpr int kSinkWaves = sizeof(T) * DP > 384 ? 2 : 4;  // float32 heads of 128: 49 KB of tiles per wave
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sinks(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
+__global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2 : 1) void window_attention_sinks(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
                                                                    AttentionShape a, int chunk, int chunks,
                                                                    const float* __restrict__ lse, const float* __restrict__ delta,
                                                                    float* __restrict__ partial) {
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sin
     };
     __shared__ union Shared {
         WaveTiles wave[kOwn];
-        float sums[kSinkSums<DP>];
+        __attribute__((aligned(16))) float sums[kSinkSums<DP>];
     } shared;
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int c = id % chunks;
@@ -202,13 +206,12 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sin
         g_next.store(tile.g);
         tile.stats[half][lane & 31] = stat;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        typename Tl::Pool pool, more;
+        typename Tl::Pool pool;
         Tl::rows(pool, tile.q);
-        Tl::rows(more, tile.g);
         v16f s = Tl::rows_times(pool, kf);
+        Tl::rows(pool, tile.g);
+        v16f dp = Tl::rows_times(pool, vf);
         Tl::cols(pool, tile.g);
-        v16f dp = Tl::rows_times(more, vf);
-        Tl::cols(more, tile.q);
         const int rows = end - i0 - 4 * half;
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
@@ -224,7 +227,8 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sin
             }
         }
         Tl::cols_times(pool, s, dv_acc);
-        Tl::cols_times(more, dp, dk_acc);
+        Tl::cols(pool, tile.q);
+        Tl::cols_times(pool, dp, dk_acc);
     }
     __syncthreads();
     for (int w = 0; w < kOwn; ++w) {
@@ -232,10 +236,13 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sin
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float* p = &shared.sums[(dt * 16 + i) * 128 + lane];
-                    p[0] = w == 0 ? dk_acc[dt][i] : p[0] + dk_acc[dt][i];
-                    p[64] = w == 0 ? dv_acc[dt][i] : p[64] + dv_acc[dt][i];
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    v4f k4, v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) k4[e] = dk_acc[dt][4 * i4 + e], v4[e] = dv_acc[dt][4 * i4 + e];
+                    v4f *pk = sink_vec<DP>(shared.sums, dt, i4, 0), *pv = sink_vec<DP>(shared.sums, dt, i4, 1);
+                    *pk = w == 0 ? k4 : *pk + k4;
+                    *pv = w == 0 ? v4 : *pv + v4;
                 }
         }
         __syncthreads();
@@ -244,13 +251,27 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>)) void window_attention_sin
     for (int i = threadIdx.x; i < kSinkSums<DP>; i += 64 * kOwn) out[i] = shared.sums[i];
 }
 
-// Keys [k0, k0 + 128) of one key/value head: the queries of the block's window, then the sums that window_attention_sinks
-// left for its sinks.
+// Adds the chunks of one block of 32 sinks (blockIdx.y) into the first of them, in order.
+template <int DP>
+__global__ __launch_bounds__(256) void window_attention_sinks_join(AttentionShape a, int chunk, int chunks, float* __restrict__ partial) {
+    const int sink_blocks = (a.sinks + 31) / 32, block = blockIdx.y % sink_blocks;
+    const int64_t seq = blockIdx.y / sink_blocks / a.kv_heads;
+    const int length = seq_length(a, seq), left = length - window_end(a, block * 32 / kBlock * kBlock, length);
+    v4f* p = reinterpret_cast<v4f*>(partial + static_cast<int64_t>(blockIdx.y) * chunks * kSinkSums<DP>) + blockIdx.x * 256 + threadIdx.x;
+    const int filled = (left + chunk - 1) / chunk;
+    if (filled <= 1) return;
+    v4f sum = *p;
+#pragma unroll 8
+    for (int n = 1; n < filled; ++n) sum += p[n * (kSinkSums<DP> / 4)];
+    *p = sum;
+}
+
+// Keys [k0, k0 + 128) of one key/value head and the queries of the block's window.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
-                                                                 AttentionShape a, float scale, int k_blocks, int chunk,
-                                                                 int chunks, const float* __restrict__ lse,
-                                                                 const float* __restrict__ delta, const float* __restrict__ partial,
+                                                                 AttentionShape a, float scale, int k_blocks, int chunks,
+                                                                 const float* __restrict__ lse, const float* __restrict__ delta,
+                                                                 float* __restrict__ partial,
                                                                  T* __restrict__ dk, T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
     constexpr int kTile = kTileRows<T>;
@@ -280,8 +301,20 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
     const int wave_last = w0 < a.sinks ? length - 1 : min(w0 + 31 + a.left, length - 1);
 
     v16f dk_acc[DP / 32], dv_acc[DP / 32];
+    if (w0 < a.sinks && end < length) {  // what the queries behind the window give the sinks
+        float* sums = partial + sink_sums<DP>(a, seq, kv_head, w0 / 32, chunks);
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const v4f k4 = *sink_vec<DP>(sums, dt, i4, 0), v4 = *sink_vec<DP>(sums, dt, i4, 1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dk_acc[dt][4 * i4 + e] = k4[e], dv_acc[dt][4 * i4 + e] = v4[e];
+            }
+    } else {
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+    }
 
     TileInFlight<T, DP, kTile, kThreads> q_next, g_next;
     q_next.place(q.token, a.dim);
@@ -349,20 +382,6 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
             Tl::cols_times(pool, dp, dk_acc);
         }
     }
-    const int sink_block = w0 / 32;
-    if (w0 < a.sinks && end < length) {
-        const int filled = (length - end + chunk - 1) / chunk;
-        const float* p = partial + sink_sums<DP>(a, seq, kv_head, sink_block, chunks) + lane_id();
-        for (int n = 0; n < filled; ++n, p += kSinkSums<DP>) {
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    dk_acc[dt][i] += p[(dt * 16 + i) * 128];
-                    dv_acc[dt][i] += p[(dt * 16 + i) * 128 + 64];
-                }
-        }
-    }
     if (__any(kept && !(all_finite(dk_acc) && all_finite(dv_acc)))) {
         const T* kr = static_cast<const T*>(k.p) + seq * k.seq + static_cast<int64_t>(mine) * k.token + kv_head * k.head;
         const T* vr = static_cast<const T*>(v.p) + seq * v.seq + static_cast<int64_t>(mine) * v.token + kv_head * v.head;
@@ -385,19 +404,21 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
     }
 }
 
-// How the queries behind the windows of the sinks are cut: chunks of 256 (two rounds of a workgroup's waves), at most 32 of
-// them, since the block of keys adds them one after the other.
+// How the queries behind the windows of the sinks are cut: chunks of 128, one round of a workgroup's waves, where all of them
+// run at once (two workgroups per CU), else of 256 (4 x 4096 x 8 x 64 bfloat16: 11.7 against 16.5 us; 4 x 2000 x 2 x 32 float32:
+// 14.4 against 9.6 us with chunks of 128); at most 32 chunks.
 struct FarPlan {
     int sink_blocks, chunk, chunks;
 };
-FarPlan far_plan(int64_t n_tokens, int64_t left, int64_t sinks) {
+FarPlan far_plan(int64_t rows, int64_t n_tokens, int64_t left, int64_t sinks) {  // rows: key/value heads of all sequences
     FarPlan f = {0, 1, 0};
     if (left > n_tokens) left = n_tokens;
     if (sinks > n_tokens) sinks = n_tokens;
     const int64_t far = n_tokens - kBlock - left;
     if (sinks <= 0 || far <= 0) return f;
-    const int64_t least = (far + 31) / 32, chunk = least <= 256 ? 256 : (least + 127) / 128 * 128;
     f.sink_blocks = static_cast<int>((sinks + 31) / 32);
+    int64_t chunk = rows * f.sink_blocks * ((far + 127) / 128) <= 512 ? 128 : 256;
+    if (chunk * 32 < far) chunk = ((far + 31) / 32 + 127) / 128 * 128;
     f.chunk = static_cast<int>(chunk);
     f.chunks = static_cast<int>((far + chunk - 1) / chunk);
     return f;
@@ -417,7 +438,7 @@ int attention_tensor(const char* name, const char* what, const void* p, const in
 extern "C" size_t mvx_window_attention_backward_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
                                                                 int64_t left, int64_t sinks) {
     if (n_seqs <= 0 || n_tokens <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || left < 0) return 0;
-    const mvx::FarPlan f = mvx::far_plan(n_tokens, left, sinks);
+    const mvx::FarPlan f = mvx::far_plan(n_seqs * kv_heads, n_tokens, left, sinks);
     const size_t rows = (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;  // delta, padded to 16 bytes
     return (rows + static_cast<size_t>(n_seqs) * kv_heads * f.sink_blocks * f.chunks * mvx::padded_dim(dim) * 64) *
            sizeof(float);
@@ -451,33 +472,41 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     const int64_t row = static_cast<int64_t>(heads) * dim;
     const TokenTensor ot = {out, n_tokens * row, row, dim};
     const int blocks = static_cast<int>((n_tokens + kBlock - 1) / kBlock);
-    const FarPlan f = far_plan(n_tokens, left, sinks);
-    MVX_REQUIRE(n_seqs <= (1 << 23) / blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23),
+    const FarPlan f = far_plan(n_seqs * kv_heads, n_tokens, left, sinks);
+    MVX_REQUIRE(n_seqs <= (1 << 23) / blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23) &&
+                    n_seqs * kv_heads * f.sink_blocks <= 65535,
                 MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch", name);
     float* delta = static_cast<float*>(workspace);
     float* partial = delta + (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
-        const auto launch = [&](auto dq_kernel, auto sinks_kernel, int sink_waves, auto dkv_kernel) {
+        const auto launch = [&](auto dq_kernel, auto sinks_kernel, int sink_waves, auto join_kernel, auto dkv_kernel) {
             const float* d = delta;
             hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * blocks)), dim3(kThreads), 0, st, qt, kt, vt,
                                ot, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
+            const unsigned sinks_of_all = static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks);
             if (f.chunks > 0)
-                hipLaunchKernelGGL(sinks_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks * f.chunks)),
-                                   dim3(64 * sink_waves), 0, st, qt, kt, vt, gt, s, f.chunk, f.chunks, lse, d, partial);
+                hipLaunchKernelGGL(sinks_kernel, dim3(sinks_of_all * f.chunks), dim3(64 * sink_waves), 0, st, qt, kt, vt, gt, s, f.chunk,
+                                   f.chunks, lse, d, partial);
+            if (f.chunks > 1)
+                hipLaunchKernelGGL(join_kernel, dim3(padded_dim(dim) * 64 / 4 / 256, sinks_of_all), dim3(256), 0, st, s, f.chunk, f.chunks,
+                                   partial);
             hipLaunchKernelGGL(dkv_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
-                               vt, gt, s, scale, blocks, f.chunk, f.chunks, lse, d, static_cast<const float*>(partial),
-                               static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+                               vt, gt, s, scale, blocks, f.chunks, lse, d, partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
         };
         if (dim <= 32)
-            launch(window_attention_dq<T, 32>, window_attention_sinks<T, 32>, kSinkWaves<T, 32>, window_attention_dkv<T, 32>);
+            launch(window_attention_dq<T, 32>, window_attention_sinks<T, 32>, kSinkWaves<T, 32>, window_attention_sinks_join<32>,
+                   window_attention_dkv<T, 32>);
         else if (dim <= 64)
-            launch(window_attention_dq<T, 64>, window_attention_sinks<T, 64>, kSinkWaves<T, 64>, window_attention_dkv<T, 64>);
+            launch(window_attention_dq<T, 64>, window_attention_sinks<T, 64>, kSinkWaves<T, 64>, window_attention_sinks_join<64>,
+                   window_attention_dkv<T, 64>);
         else if (dim <= 96)
-            launch(window_attention_dq<T, 96>, window_attention_sinks<T, 96>, kSinkWaves<T, 96>, window_attention_dkv<T, 96>);
+            launch(window_attention_dq<T, 96>, window_attention_sinks<T, 96>, kSinkWaves<T, 96>, window_attention_sinks_join<96>,
+                   window_attention_dkv<T, 96>);
         else
-            launch(window_attention_dq<T, 128>, window_attention_sinks<T, 128>, kSinkWaves<T, 128>, window_attention_dkv<T, 128>);
+            launch(window_attention_dq<T, 128>, window_attention_sinks<T, 128>, kSinkWaves<T, 128>, window_attention_sinks_join<128>,
+                   window_attention_dkv<T, 128>);
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });
