@@ -11,6 +11,9 @@
 // are therefore cut into chunks that a third kernel takes, between the two: a workgroup per chunk and 32 sinks, its waves
 // on queries of their own, its sum left in float32.  A fourth adds the chunks in order, and the block of keys starts from that.
 // p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.
+// A query that sees a single key weighs it with 1 whatever its score: dp - delta is zero there, but rounding would leave noise,
+// which is all there is where every query sees one key.  The first kernel counts the keys a query sees, gives such a query no
+// gradient, and leaves a mark in the place of its delta.
 #include "attention_tiles.h"
 
 namespace mvx {
@@ -18,6 +21,13 @@ namespace mvx {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlock = 32 * kWaves;
+
+// In the place of a query's delta: it sees a single key.  A NaN of its own, which no arithmetic makes.
+constexpr unsigned kAlone = 0x7fe5a10eu;
+__device__ __forceinline__ bool is_alone(float delta) { return __builtin_bit_cast(unsigned, delta) == kAlone; }
+
+// The lowest n bits.
+__device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
@@ -53,10 +63,23 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
                                         a.dim, live));
     const int64_t at_row = (seq * a.heads + head) * a.n_tokens + mine;
     if (live) my_lse = lse[at_row];
-    if (mine < a.n_tokens && half == 0) delta[at_row] = my_delta;
 
     const int hi = live ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
     const KeyTiles tiles = key_tiles(a, q0, kBlock, length, kTile);
+    // Counted ahead of the products, which have no registers left (counting along with them took 3 to 6 % more time).
+    int n_seen = max(0, hi + 1 - max(lo, 0)) + max(0, min(min(a.sinks, hi + 1), lo));
+    if (a.visible != nullptr) {
+        n_seen = 0;
+        for (int t = 0; t < tiles.count && __any(live && n_seen < 2); ++t) {
+            const int k0 = tiles.key0(t, kTile);
+            const uint64_t keep = __ballot(token_kept(a, seq, k0, length)) & below(kTile);
+            n_seen += __popcll(keep & below(hi + 1 - k0) & (~below(lo - k0) | below(a.sinks - k0)));
+        }
+    }
+    // not where the key or what it gave is infinite or NaN: 0 times that is NaN
+    const bool alone = n_seen == 1 && __builtin_isfinite(my_lse) && __builtin_isfinite(my_delta);
+    if (mine < a.n_tokens && half == 0) delta[at_row] = alone ? __builtin_bit_cast(float, kAlone) : my_delta;
+    if (alone) my_lse = __builtin_inff();  // weights of zero: no gradient
     v16f acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
@@ -223,7 +246,7 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e])), ds = p * (dp[i] - d4[e]);
                 const bool seen = kept && 8 * i4 + e < rows;
                 s[i] = seen ? p : 0.0f;
-                dp[i] = seen ? ds : 0.0f;
+                dp[i] = seen && !is_alone(d4[e]) ? ds : 0.0f;
             }
         }
         Tl::cols_times(pool, s, dv_acc);
@@ -369,12 +392,13 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
                 }
             }
             if (!whole) {
+                const unsigned alone = static_cast<unsigned>(__ballot(is_alone(stats[t & 1][1][32 * b + (lane_id() & 31)]))) >> (4 * half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = 32 * b + 8 * (i / 4) + i % 4;
+                    const int e = 8 * (i / 4) + i % 4, r = 32 * b + e;
                     const bool seen = r >= lo_r && r <= hi_r;
                     s[i] = seen ? s[i] : 0.0f;
-                    dp[i] = seen ? dp[i] : 0.0f;
+                    dp[i] = seen && !((alone >> e) & 1) ? dp[i] : 0.0f;
                 }
             }
             Tl::cols_times(pool, s, dv_acc);
@@ -393,7 +417,7 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
                 const T* gr = static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(i) * g.token + h * g.head;
                 const int64_t at = (seq * a.heads + h) * a.n_tokens + i;
                 const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, kr, a.dim), a.scale_log2, -lse[at]));
-                add_row<T, DP>(dk_acc, p * (dot_rows(gr, vr, a.dim) - delta[at]), qr, a.dim);
+                if (!is_alone(delta[at])) add_row<T, DP>(dk_acc, p * (dot_rows(gr, vr, a.dim) - delta[at]), qr, a.dim);
                 add_row<T, DP>(dv_acc, p, gr, a.dim);
             }
     }

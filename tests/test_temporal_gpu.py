@@ -587,3 +587,38 @@ def test_refusals_on_the_gpu():
         temporal.window_cache_fill(t, t, torch.zeros(2, 5, 4, 16, device=DEV), torch.zeros(2, 6, 4, 16, device=DEV), n)
     with pytest.raises(ValueError, match="k_cache"):
         temporal.window_cache_fill(t, t, cache, cache.clone(), n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window,sinks,hidden", [((0, 0), 0, False), ((0, 0), 0, True), ((3, 0), 1, True), ((0, 0), 2, False)])
+def test_a_query_that_sees_one_key_gives_q_and_k_no_gradient(dtype, window, sinks, hidden):
+    """Its weight is 1 whatever the score; what rounding leaves of dp - delta must not pass for a gradient."""
+    n = 420
+    g = gen(51)
+    q, k, v = (normal(g, (2, n, heads, 32), dtype, True) for heads in (4, 2, 2))
+    up = normal(g, (2, n, 4, 32), dtype)
+    visible = torch.rand((2, n), generator=g) < 0.25 if hidden else None
+    lengths = torch.tensor([n, 333])
+    out = temporal.window_attention(q, k, v, window, sinks, lengths=on_gpu(lengths), visible=on_gpu(visible))
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), up)
+    want, bound, grads, bounds = orc.attention(f64(q), f64(k), f64(v), window, sinks, dtype, lengths, visible, grad=f64(up))
+    for name, a, c, e in zip(("dq", "dk", "dv"), (dq, dk, dv), grads, bounds):
+        within(a, c, e, name)
+    for s in range(2):
+        seen = orc.seen_pairs(n, *window, sinks, int(lengths[s]), None if visible is None else visible[s])
+        alone = seen.sum(-1) == 1
+        assert alone.any() and (dq[s, alone] == 0).all()
+        only_theirs = ~seen[seen.sum(-1) > 1].any(0)  # keys that no query with a choice sees
+        assert (dk[s, only_theirs] == 0).all()
+
+
+def test_a_query_whose_only_key_is_not_finite_does_not_hide_it():
+    q, k, v = (normal(gen(52), (1, 40, 2, 32), torch.float32) for _ in range(3))
+    k[0, 7, 0, 3] = float("nan")
+    v[0, 20, 1, 3] = float("inf")
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = temporal.window_attention(q, k, v, (0, 0))
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    assert dq[0, 7, 0].isnan().all() and dk[0, 7, 0].isnan().all() and dq[0, 20, 1].isnan().all()
+    dq[0, 7, 0] = dk[0, 7, 0] = dq[0, 20, 1] = dk[0, 20, 1] = 0
+    assert (dq == 0).all() and (dk == 0).all()
