@@ -409,17 +409,19 @@ int mvx_rotate_positions(const void* q, const int64_t* q_strides, int q_heads, c
  * left, right  >= 0; values beyond n_tokens mean no limit
  * lengths      [n_seqs] int64 or NULL (values outside 0 .. n_tokens are clamped);  visible [n_seqs][n_tokens] bytes or NULL
  * out          [n_seqs][n_tokens][heads][dim], contiguous
- * lse          [n_seqs][heads][n_tokens] float32 out: log2 of the softmax denominator, what the backward reads; or NULL
+ * saved        out: what the backward reads (log2 of the softmax denominators and, with 16-bit types, what the rounding of out
+ *              left): mvx_window_attention_saved_bytes() bytes, 16-byte aligned; or NULL
  */
+size_t mvx_window_attention_saved_bytes(int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int dim);
 int mvx_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                          const int64_t* v_strides, int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
                          int64_t left, int64_t right, int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
-                         void* out, float* lse, void* stream);
+                         void* out, void* saved, void* stream);
 
 /*
  * Backward of mvx_window_attention: gradients of q, k and v given grad_out.  Summed in a fixed order, no atomics; tokens at or
  * behind a sequence's length, and keys that are hidden, get zeros.
- * out, lse        what the forward call wrote
+ * out, saved      what the forward call wrote
  * grad_out        as q: [n_seqs][n_tokens][heads][dim] with strides
  * grad_q          [n_seqs][n_tokens][heads][dim]; grad_k, grad_v [n_seqs][n_tokens][kv_heads][dim]; contiguous
  * workspace       mvx_window_attention_backward_workspace_bytes() bytes, 16-byte aligned
@@ -427,7 +429,7 @@ int mvx_window_attention(const void* q, const int64_t* q_strides, const void* k,
 size_t mvx_window_attention_backward_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int heads, int kv_heads, int dim,
                                                      int64_t left, int64_t sinks);
 int mvx_window_attention_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                                  const void* v, const int64_t* v_strides, const void* out, const float* lse,
+                                  const void* v, const int64_t* v_strides, const void* out, const void* saved,
                                   const void* grad_out, const int64_t* grad_strides, int dtype, int64_t n_seqs,
                                   int64_t n_tokens, int heads, int kv_heads, int dim, int64_t left, int64_t right,
                                   int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible, void* grad_q,

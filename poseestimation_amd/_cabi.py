@@ -66,6 +66,7 @@ SIGNATURES = {
                                     ctypes.c_double, _int, _int, _int, _vp, _vp, _vp]),
     "mvx_window_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _f32,
                                     _vp, _vp, _vp, _vp, _vp]),
+    "mvx_window_attention_saved_bytes": (_sz, [_int, _i64, _i64, _int, _int]),
     "mvx_window_attention_backward_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int, _i64, _i64]),
     "mvx_window_attention_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _int, _int,
                                              _int, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -141,6 +141,22 @@ struct Tiles16 {
             for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mfma(p.a[s * (DP / 32) + dt], b, acc[dt]);
         }
     }
+    // start + the sum of the weights as cols_times rounds them
+    static __device__ __forceinline__ float rounded_sum(const v16f& w, float start) {
+        typedef T v2 __attribute__((ext_vector_type(2)));
+        const v2 one = {static_cast<T>(1.0f), static_cast<T>(1.0f)};
+        float sum[2] = {start, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const v2 b = {static_cast<T>(w[i]), static_cast<T>(w[i + 1])};
+            float& s = sum[i / 2 % 2];
+            if constexpr (std::is_same_v<T, bf16>)
+                s = __builtin_amdgcn_fdot2_f32_bf16(b, one, s, false);
+            else
+                s = __builtin_amdgcn_fdot2(b, one, s, false);
+        }
+        return sum[0] + sum[1];
+    }
 };
 template <int DP>
 struct Tiles<bf16, DP> : Tiles16<bf16, DP> {};
@@ -245,9 +261,10 @@ struct Tiles<float, DP> {
 template <typename T>
 constexpr int kTileRows = sizeof(T) == 4 ? 32 : 64;
 
-// This half's share of the product of two rows, in the columns that load_column gives it.
+// This half's share of the product of a row and the sum of two (of float32: the first of them), in the columns that load_column
+// gives it.
 template <typename T>
-__device__ __forceinline__ float half_dot(const T* a, const T* b, int dim, bool valid) {
+__device__ __forceinline__ float half_dot(const T* a, const T* b, const T* rest, int dim, bool valid) {
     float r = 0.0f;
     if (valid)
         for (int d = 8 * (lane_id() >> 5); d < dim; d += 16)
@@ -256,6 +273,12 @@ __device__ __forceinline__ float half_dot(const T* a, const T* b, int dim, bool 
                 float x[Element<T>::vec], y[Element<T>::vec];
                 load_vec<T>(a + d + e, x);
                 load_vec<T>(b + d + e, y);
+                if constexpr (sizeof(T) == 2) {
+                    float z[Element<T>::vec];
+                    load_vec<T>(rest + d + e, z);
+#pragma unroll
+                    for (int i = 0; i < Element<T>::vec; ++i) y[i] += z[i];
+                }
 #pragma unroll
                 for (int i = 0; i < Element<T>::vec; ++i) r = fmaf(x[i], y[i], r);
             }
@@ -322,9 +345,10 @@ struct TileInFlight {
     }
 };
 
-// Stores the lane's column of a 32 x DP block of sums: times `factor`, the first `dim` values of `row`.
+// Stores the lane's column of a 32 x DP block of sums: times `factor`, the first `dim` values of `row`.  `rest`, where
+// given, takes what this rounding to T left of them.
 template <typename T, int DP>
-__device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float factor, T* row, int dim) {
+__device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float factor, T* row, int dim, T* rest = nullptr) {
     typedef T vec4 __attribute__((ext_vector_type(4)));
     const int half = lane_id() >> 5;
 #pragma unroll
@@ -333,14 +357,29 @@ __device__ __forceinline__ void store_columns(const v16f (&acc)[DP / 32], float 
         for (int b = 0; b < 4; ++b) {
             const int d = 32 * dt + 8 * b + 4 * half;
             if (d >= dim) continue;
+            float x[4];
             vec4 w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[dt][4 * b + e] * factor);
+            for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(x[e] = acc[dt][4 * b + e] * factor);
+            // one rounding for both: made twice, by a conversion and inside a product, near ties fell to either side
+            unsigned pair[sizeof(w) / 4];
+            __builtin_memcpy(pair, &w, sizeof(w));
+#pragma unroll
+            for (unsigned& p : pair) asm("" : "+v"(p));
+            __builtin_memcpy(&w, pair, sizeof(w));
             *reinterpret_cast<vec4*>(row + d) = w;
+            if (rest == nullptr) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float left = x[e] - static_cast<float>(w[e]);
+                w[e] = static_cast<T>(__builtin_isfinite(left) ? left : 0.0f);
+            }
+            *reinterpret_cast<vec4*>(rest + d) = w;
         }
 }
 
 // What the attention entry points share.
+inline int64_t padded_rows(int64_t rows) { return (rows + 3) / 4 * 4; }  // a float per row, and what follows aligned to 16 bytes
 struct TokenTensor {
     const void* p;
     int64_t seq, token, head;  // strides in elements

@@ -8,8 +8,10 @@
 // softmax of a query runs inside a lane and its partner 32 lanes on, with a running maximum and sum, and the weighted sum of
 // the values takes the scores where they lie.  A tile is held in LDS for all waves and the next one travels from memory
 // meanwhile; tiles that every query sees whole skip the mask, and a wave skips a tile that none of its queries sees.
-// Scores and sums are float32; the weights (at most 1) are rounded to the element type for the second product, the sum that
-// divides the result is taken before that rounding.
+// Scores and sums are float32; the weights (at most 2^kSlack) are rounded to the element type for the second product.  The sum
+// that divides the result is that of the rounded weights: the result is a mean of the values whose weights are off by relative
+// errors alone, so a row that one key dominates is as exact as that key's value, which the backward's differences need.  What
+// the backward takes the weights from, the logarithm of the sum, is that of the weights before rounding.
 #include "attention_tiles.h"
 
 namespace mvx {
@@ -21,7 +23,7 @@ constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2
 // The registers are cut for two waves per SIMD where they suffice: with one, a long prompt of heads of 128 took 1.8 times as long.
 template <typename T, int DP, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
-    TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse) {
+    TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest) {
     using Tl = Tiles<T, DP>;
     constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = kWaves == 1 ? 32 : kTileRows<T>;  // queries of the workgroup, keys of a tile
     __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kBK * Tl::LD];
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
     v16f acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
-    float top = -kInf, sum = 0.0f;
+    float top = -kInf, sum = 0.0f, divisor = 0.0f;
 
     const KeyTiles tiles = key_tiles(a, q0, kBQ, length, kBK);
     TileInFlight<T, DP, kBK, 64 * kWaves> k_next, v_next;
@@ -122,21 +124,25 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
             if (__any(most > top + kSlack)) {
                 const float next = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - (next == -kInf ? 0.0f : next));
                 sum *= f;
+                divisor *= f;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;  // top = -inf: 0
                 top = next;
             }
             const float ref = top == -kInf ? 0.0f : top;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -ref));
-                sum += s[i];
-            }
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -ref));
             Tl::cols_times(pool, s, acc);
+            if constexpr (sizeof(T) == 2) divisor = Tl::rounded_sum(s, divisor);
+            if (sizeof(T) == 4 || lse != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += s[i];
+            }
         }
     }
     sum = both_halves_sum(sum);
-    if (__any(mine < length && !(all_finite(acc) && sum < kInf))) {
+    divisor = sizeof(T) == 2 ? both_halves_sum(divisor) : sum;
+    if (__any(mine < length && !(all_finite(acc) && divisor < kInf))) {
         const T* qr = qb + static_cast<int64_t>(mine) * q.token;
         top = -kInf;
         sum = 0.0f;
@@ -151,12 +157,15 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
             sum += p;
             add_row<T, DP>(acc, p, vb + j * v.token, a.dim);
         });
+        divisor = sum;
     }
     if (mine >= a.n_tokens) return;
     const bool none = top == -kInf;
     if (lse != nullptr && half == 0)
         lse[(seq * a.heads + head) * a.n_tokens + mine] = none ? 0.0f : top + __builtin_amdgcn_logf(sum);  // log2
-    store_columns<T, DP>(acc, none ? 0.0f : 1.0f / sum, out + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim);
+    const float factor = none ? 0.0f : 1.0f / divisor;
+    const int64_t row = ((seq * a.n_tokens + mine) * a.heads + head) * a.dim;
+    store_columns<T, DP>(acc, factor, out + row, a.dim, sizeof(T) == 2 && lse != nullptr ? rest + row : nullptr);
 }
 
 }  // namespace
@@ -199,10 +208,16 @@ int attention_tensor(const char* name, const char* what, const void* p, const in
 
 }  // namespace mvx
 
+extern "C" size_t mvx_window_attention_saved_bytes(int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int dim) {
+    if (n_seqs <= 0 || n_tokens <= 0 || heads <= 0 || dim <= 0) return 0;
+    const int64_t rows = n_seqs * n_tokens * heads;
+    return static_cast<size_t>(mvx::padded_rows(rows)) * sizeof(float) + (dtype == MVX_F32 ? 0 : static_cast<size_t>(rows) * dim * 2);
+}
+
 extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                     const void* v, const int64_t* v_strides, int dtype, int64_t n_seqs, int64_t n_tokens,
                                     int heads, int kv_heads, int dim, int64_t left, int64_t right, int64_t sinks, float scale,
-                                    const int64_t* lengths, const uint8_t* visible, void* out, float* lse, void* stream) {
+                                    const int64_t* lengths, const uint8_t* visible, void* out, void* saved, void* stream) {
     using namespace mvx;
     const char* name = "mvx_window_attention";
     AttentionShape s;
@@ -214,6 +229,8 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &kt)) != MVX_OK) return rc;
     if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
     MVX_REQUIRE(out != nullptr && aligned16(out), MVX_ERR_INVALID_ARGUMENT, "%s: out is null or not 16-byte aligned", name);
+    MVX_REQUIRE(aligned16(saved), MVX_ERR_INVALID_ARGUMENT, "%s: saved is not 16-byte aligned", name);
+    float* lse = static_cast<float*>(saved);
     // Four waves share their tiles, and wait for each other's: of a window of w keys a wave sees 32 + w, the workgroup 128 + w.
     // Short windows are therefore walked by single waves where their tiles leave room for enough of them: always with 16-bit
     // types (4 x 4096 tokens x 8 heads x 64, 33 keys: 22.8 -> 20.7 us; from 255 keys on four waves are faster), with float32, whose
@@ -230,7 +247,7 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
         using T = decltype(zero);
         const auto launch = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
-                               static_cast<T*>(out), lse);
+                               static_cast<T*>(out), lse, reinterpret_cast<T*>(lse != nullptr ? lse + padded_rows(n_seqs * heads * n_tokens) : nullptr));
         };
         if (dim <= 32)
             waves == 1 ? launch(window_attention<T, 32, 1>) : launch(window_attention<T, 32, 4>);

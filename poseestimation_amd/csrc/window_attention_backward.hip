@@ -10,6 +10,9 @@
 // In the second a block of sink keys is seen by the whole rest of the sequence.  The queries behind the block's own window
 // are therefore cut into chunks that a third kernel takes, between the two: a workgroup per chunk and 32 sinks, its waves
 // on queries of their own, its sum left in float32.  A fourth adds the chunks in order, and the block of keys starts from that.
+// delta is taken from the output together with what its rounding left: a row that one key dominates has dp - delta near zero
+// there, and the output rounded to bfloat16 alone would be off by as much as the difference (three keys of unit spread: dq and dk
+// off by 0.0033 of their size instead of 0.0025, of twice that spread 0.0066 instead of 0.0024).
 // p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.
 // A query that sees a single key weighs it with 1 whatever its score: dp - delta is zero there, but rounding would leave noise,
 // which is all there is where every query sees one key.  The first kernel counts the keys a query sees, gives such a query no
@@ -31,7 +34,7 @@ __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
-                                                                TokenTensor g, AttentionShape a, float scale, int q_blocks,
+                                                                const T* __restrict__ rest, TokenTensor g, AttentionShape a, float scale, int q_blocks,
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
                                                                 T* __restrict__ dq) {
     using Tl = Tiles<T, DP>;
@@ -60,7 +63,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     float my_lse = 0.0f;
     const float my_delta = both_halves_sum(half_dot(static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head,
                                         static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head,
-                                        a.dim, live));
+                                        rest + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim, live));
     const int64_t at_row = (seq * a.heads + head) * a.n_tokens + mine;
     if (live) my_lse = lse[at_row];
 
@@ -463,13 +466,13 @@ extern "C" size_t mvx_window_attention_backward_workspace_bytes(int64_t n_seqs, 
                                                                 int64_t left, int64_t sinks) {
     if (n_seqs <= 0 || n_tokens <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || left < 0) return 0;
     const mvx::FarPlan f = mvx::far_plan(n_seqs * kv_heads, n_tokens, left, sinks);
-    const size_t rows = (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;  // delta, padded to 16 bytes
+    const size_t rows = mvx::padded_rows(n_seqs * heads * n_tokens);  // delta
     return (rows + static_cast<size_t>(n_seqs) * kv_heads * f.sink_blocks * f.chunks * mvx::padded_dim(dim) * 64) *
            sizeof(float);
 }
 
 extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                                             const void* v, const int64_t* v_strides, const void* out, const float* lse,
+                                             const void* v, const int64_t* v_strides, const void* out, const void* saved,
                                              const void* grad_out, const int64_t* grad_strides, int dtype, int64_t n_seqs,
                                              int64_t n_tokens, int heads, int kv_heads, int dim, int64_t left, int64_t right,
                                              int64_t sinks, float scale, const int64_t* lengths, const uint8_t* visible,
@@ -486,10 +489,10 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     if ((rc = attention_tensor(name, "k", k, k_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &kt)) != MVX_OK) return rc;
     if ((rc = attention_tensor(name, "v", v, v_strides, dtype, n_seqs, n_tokens, kv_heads, dim, &vt)) != MVX_OK) return rc;
     if ((rc = attention_tensor(name, "grad_out", grad_out, grad_strides, dtype, n_seqs, n_tokens, heads, dim, &gt)) != MVX_OK) return rc;
-    MVX_REQUIRE(out != nullptr && lse != nullptr && grad_q != nullptr && grad_k != nullptr && grad_v != nullptr,
+    MVX_REQUIRE(out != nullptr && saved != nullptr && grad_q != nullptr && grad_k != nullptr && grad_v != nullptr,
                 MVX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
-    MVX_REQUIRE(aligned16(out) && aligned16(grad_q) && aligned16(grad_k) && aligned16(grad_v) && aligned16(workspace),
-                MVX_ERR_INVALID_ARGUMENT, "%s: out, the gradients and the workspace must be 16-byte aligned", name);
+    MVX_REQUIRE(aligned16(out) && aligned16(saved) && aligned16(grad_q) && aligned16(grad_k) && aligned16(grad_v) && aligned16(workspace),
+                MVX_ERR_INVALID_ARGUMENT, "%s: out, saved, the gradients and the workspace must be 16-byte aligned", name);
     const size_t need = mvx_window_attention_backward_workspace_bytes(n_seqs, n_tokens, heads, kv_heads, dim, left, sinks);
     MVX_REQUIRE(workspace != nullptr && workspace_bytes >= need, MVX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu",
                 name, need, workspace_bytes);
@@ -501,14 +504,15 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
                     n_seqs * kv_heads * f.sink_blocks <= 65535,
                 MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch", name);
     float* delta = static_cast<float*>(workspace);
-    float* partial = delta + (static_cast<size_t>(n_seqs) * heads * n_tokens + 3) / 4 * 4;
+    float* partial = delta + padded_rows(n_seqs * heads * n_tokens);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
         const auto launch = [&](auto dq_kernel, auto sinks_kernel, int sink_waves, auto join_kernel, auto dkv_kernel) {
-            const float* d = delta;
+            const float *d = delta, *lse = static_cast<const float*>(saved);
+            const T* rest = reinterpret_cast<const T*>(lse + padded_rows(n_seqs * heads * n_tokens));
             hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * blocks)), dim3(kThreads), 0, st, qt, kt, vt,
-                               ot, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
+                               ot, rest, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
             const unsigned sinks_of_all = static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks);
             if (f.chunks > 0)
                 hipLaunchKernelGGL(sinks_kernel, dim3(sinks_of_all * f.chunks), dim3(64 * sink_waves), 0, st, qt, kt, vt, gt, s, f.chunk,

@@ -306,29 +306,31 @@ def _tokens(t):
     return c if c.data_ptr() % 16 == 0 else c.clone()
 
 
-def _window_run(q, k, v, lengths, visible, how, want_lse):
+def _window_run(q, k, v, lengths, visible, how, for_backward):
     q, k, v = _tokens(q), _tokens(k), _tokens(v)
     b, n, heads, dim = q.shape
     out = torch.empty((b, n, heads, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, heads, n), dtype=torch.float32, device=q.device) if want_lse else None
+    saved = None
+    if for_backward:
+        saved = _workspace(_cabi.load().mvx_window_attention_saved_bytes(_DTYPES[q.dtype], b, n, heads, dim), q.device)
     _run(q.get_device(), "window_attention", "mvx_window_attention", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
          v.data_ptr(), _strides(v), _DTYPES[q.dtype], b, n, heads, k.shape[2], dim, *how, _pointer(lengths), _pointer(visible),
-         out.data_ptr(), _pointer(lse))
-    return q, k, v, out, lse
+         out.data_ptr(), _pointer(saved))
+    return q, k, v, out, saved
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, visible, how):
-        q, k, v, out, lse = _window_run(q, k, v, lengths, visible, how, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths, visible)
+        q, k, v, out, saved = _window_run(q, k, v, lengths, visible, how, True)
+        ctx.save_for_backward(q, k, v, out, saved, lengths, visible)
         ctx.how = how
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, lengths, visible = ctx.saved_tensors
+        q, k, v, out, saved, lengths, visible = ctx.saved_tensors
         left, right, sinks, scale = ctx.how
         b, n, heads, dim = q.shape
         kv_heads = k.shape[2]
@@ -338,7 +340,7 @@ class _WindowAttention(torch.autograd.Function):
         grad_v = torch.empty_like(grad_k)
         ws = _workspace(_cabi.load().mvx_window_attention_backward_workspace_bytes(b, n, heads, kv_heads, dim, left, sinks), q.device)
         _run(q.get_device(), "window_attention", "mvx_window_attention_backward", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-             v.data_ptr(), _strides(v), out.data_ptr(), lse.data_ptr(), grad.data_ptr(), _strides(grad), _DTYPES[q.dtype], b, n,
+             v.data_ptr(), _strides(v), out.data_ptr(), saved.data_ptr(), grad.data_ptr(), _strides(grad), _DTYPES[q.dtype], b, n,
              heads, kv_heads, dim, left, right, sinks, scale, _pointer(lengths), _pointer(visible), grad_q.data_ptr(),
              grad_k.data_ptr(), grad_v.data_ptr(), ws.data_ptr(), ws.numel())
         need = ctx.needs_input_grad

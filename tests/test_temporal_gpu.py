@@ -622,3 +622,35 @@ def test_a_query_whose_only_key_is_not_finite_does_not_hide_it():
     assert dq[0, 7, 0].isnan().all() and dk[0, 7, 0].isnan().all() and dq[0, 20, 1].isnan().all()
     dq[0, 7, 0] = dk[0, 7, 0] = dq[0, 20, 1] = dk[0, 20, 1] = 0
     assert (dq == 0).all() and (dk == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_of_rows_that_one_key_dominates(dtype):
+    """Two keys of weights w, 1 - w: ds = +-w (1 - w) (dp1 - dp2), of which nothing but a relative part may be lost.  With half a
+    step u: u for the rounding of ds; p times the error of delta = g . o, where the weights' roundings move o by at most
+    2 u w (1 - w) (v1 - v2) and so delta by at most 2 u |ds|; u^2 |g| |o| of what two roundings leave of o.  The float32 parts
+    (scores of up to 100, sums of 64) are within 2^-15 of ds.  Below the type's smallest normal value (2^-14 in float16) a step
+    does not shrink any more: a rounding is off by up to half a step h there, so ds and the results by h more, a weight by h of
+    the row's largest and so delta by 2 h |dp1 - dp2|, and each value that rounding left of o by h."""
+    n, dim = 700, 64
+    g = gen(53)
+    q, k = (normal(g, (1, n, 2, dim), dtype, True, spread=2.0) for _ in range(2))
+    v = normal(g, (1, n, 2, dim), dtype, True)
+    up = normal(g, (1, n, 2, dim), dtype)
+    got = torch.autograd.grad(temporal.window_attention(q, k, v, (1, 0)), (q, k), up)
+    u, scale = torch.finfo(dtype).eps / 2, dim ** -0.5
+    h = torch.finfo(dtype).tiny * u
+    q, k, v, up = (f64(t)[0].transpose(0, 1) for t in (q, k, v, up))
+    i = torch.arange(n)
+    seen = (i[None] <= i[:, None]) & (i[None] >= i[:, None] - 1)
+    p = torch.softmax((q @ k.transpose(1, 2) * scale).masked_fill(~seen, -1e300), -1)
+    out, dp = p @ v, up @ v.transpose(1, 2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    off = (3 * u + 2 ** -15) * ds.abs() + p * (u * u * (up.abs() * out.abs()).sum(-1, keepdim=True))
+    apart = (dp - torch.roll(dp, 1, 2)).abs().masked_fill(~seen, 0).amax(-1, keepdim=True)
+    off = off + h + p * (2 * h * apart + h * up.abs().sum(-1, keepdim=True))
+    off = off * (1 + 4 * u) + p * 2 ** -20 * (up.abs() @ v.abs().transpose(1, 2)).masked_fill(~seen, 0).amax(-1, keepdim=True)
+    for name, a, s, o, other in (("dq", got[0], ds, off, k), ("dk", got[1], ds.transpose(1, 2), off.transpose(1, 2), q)):
+        want = s @ other * scale
+        bound = o @ other.abs() * scale
+        within(a, want.transpose(0, 1)[None], (bound + u * (want.abs() + bound) + h).transpose(0, 1)[None], name)
