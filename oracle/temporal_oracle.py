@@ -96,7 +96,7 @@ def attention(q, k, v, window, sinks, dtype, lengths=None, visible=None, scale=N
     share = heads // k.shape[2]
     scale = dim ** -0.5 if scale is None else scale
     u = half_step(dtype)
-    flat = 2.0 ** -25 if dtype == torch.float16 else 0.0  # float16 weights below 2^-14 are rounded to multiples of 2^-24
+    flat = 2.0 ** -25 if dtype == torch.float16 else 0.0  # float16 values below 2^-14 are rounded to multiples of 2^-24
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
     grads = [torch.zeros_like(t) for t in (q, k, v)]
     bounds = [torch.zeros_like(t) for t in (q, k, v)]
@@ -120,7 +120,7 @@ def attention(q, k, v, window, sinks, dtype, lengths=None, visible=None, scale=N
             pv = p @ vh.abs()
             out[s, :, h] = o
             low = flat * seen.double() @ vh.abs()
-            bound[s, :, h] = u * (o.abs() + pv) + (rel + n * E) * pv + low
+            bound[s, :, h] = u * (o.abs() + pv) + (rel + n * E) * pv + low + flat
             if grad is None:
                 continue
             g = torch.where(some, grad[s, :, h], 0.0)
@@ -141,7 +141,7 @@ def attention(q, k, v, window, sinks, dtype, lengths=None, visible=None, scale=N
     if grad is None:
         return out, bound
     for g, e in zip(grads, bounds):
-        e += u * g.abs()
+        e += u * g.abs() + flat
     return out, bound, tuple(grads), tuple(bounds)
 
 

@@ -157,6 +157,16 @@ struct Tiles16 {
         }
         return sum[0] + sum[1];
     }
+    // this half's share of the product of a column and the sum of two
+    static __device__ __forceinline__ float dot(const Frag& f, const Frag& g, const Frag& rest) {
+        float r = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                r = fmaf(static_cast<float>(f.step[s][i]), static_cast<float>(g.step[s][i]) + static_cast<float>(rest.step[s][i]), r);
+        return r;
+    }
 };
 template <int DP>
 struct Tiles<bf16, DP> : Tiles16<bf16, DP> {};
@@ -261,26 +271,16 @@ struct Tiles<float, DP> {
 template <typename T>
 constexpr int kTileRows = sizeof(T) == 4 ? 32 : 64;
 
-// This half's share of the product of a row and the sum of two (of float32: the first of them), in the columns that load_column
-// gives it.
-template <typename T>
-__device__ __forceinline__ float half_dot(const T* a, const T* b, const T* rest, int dim, bool valid) {
+// This half's share of the product of two float32 rows, in the columns that load_column gives it.
+__device__ __forceinline__ float half_dot(const float* a, const float* b, int dim, bool valid) {
     float r = 0.0f;
     if (valid)
         for (int d = 8 * (lane_id() >> 5); d < dim; d += 16)
 #pragma unroll
-            for (int e = 0; e < 8; e += Element<T>::vec) {
-                float x[Element<T>::vec], y[Element<T>::vec];
-                load_vec<T>(a + d + e, x);
-                load_vec<T>(b + d + e, y);
-                if constexpr (sizeof(T) == 2) {
-                    float z[Element<T>::vec];
-                    load_vec<T>(rest + d + e, z);
+            for (int e = 0; e < 8; e += 4) {
+                const v4f x = *reinterpret_cast<const v4f*>(a + d + e), y = *reinterpret_cast<const v4f*>(b + d + e);
 #pragma unroll
-                    for (int i = 0; i < Element<T>::vec; ++i) y[i] += z[i];
-                }
-#pragma unroll
-                for (int i = 0; i < Element<T>::vec; ++i) r = fmaf(x[i], y[i], r);
+                for (int i = 0; i < 4; ++i) r = fmaf(x[i], y[i], r);
             }
     return r;
 }

@@ -61,9 +61,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     Tl::load_column(qf, static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head, a.dim, live);
     Tl::load_column(gf, static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head, a.dim, live);
     float my_lse = 0.0f;
-    const float my_delta = both_halves_sum(half_dot(static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head,
-                                        static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head,
-                                        rest + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim, live));
+    const T* o_row = static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head;
+    float my_delta;
+    if constexpr (sizeof(T) == 2) {
+        typename Tl::Frag of, rf;
+        Tl::load_column(of, o_row, a.dim, live);
+        Tl::load_column(rf, rest + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim, live);
+        my_delta = both_halves_sum(Tl::dot(gf, of, rf));
+    } else {
+        my_delta = both_halves_sum(half_dot(static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head, o_row, a.dim, live));
+    }
     const int64_t at_row = (seq * a.heads + head) * a.n_tokens + mine;
     if (live) my_lse = lse[at_row];
 

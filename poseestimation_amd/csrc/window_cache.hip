@@ -431,7 +431,7 @@ int check_cache(const char* name, int dtype, int64_t n_seqs, int kv_heads, int d
                 (long long)window, (long long)sinks);
     MVX_REQUIRE(dim > 0 && dim % 8 == 0, MVX_ERR_INVALID_ARGUMENT, "%s: head dimension %d is not a multiple of 8", name, dim);
     MVX_REQUIRE(dim <= 128, MVX_ERR_UNSUPPORTED, "%s: head dimension %d above 128", name, dim);
-    MVX_REQUIRE(n_seqs <= 65535 && kv_heads <= 4096 && window + sinks <= (1 << 30), MVX_ERR_UNSUPPORTED,
+    MVX_REQUIRE(n_seqs <= 65535 && kv_heads <= 4096 && window <= (1 << 30) && sinks <= (1 << 30) - window, MVX_ERR_UNSUPPORTED,
                 "%s: more than 65535 streams, 4096 heads or 2^30 slots", name);
     return MVX_OK;
 }
@@ -446,7 +446,7 @@ int attention_tensor(const char* name, const char* what, const void* p, const in
 extern "C" size_t mvx_window_attention_step_workspace_bytes(int dtype, int64_t n_seqs, int heads, int kv_heads, int dim,
                                                             int64_t window, int64_t sinks) {
     if (n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0 || window <= 0 || sinks < 0 ||
-        window + sinks > (1 << 30))
+        window > (1 << 30) || sinks > (1 << 30) - window)
         return 0;
     return static_cast<size_t>(n_seqs) * heads *
            mvx::step_shares(n_seqs, heads, kv_heads, static_cast<int>(window + sinks), dtype) * (dim + 2) * sizeof(float);

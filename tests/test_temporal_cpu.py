@@ -144,3 +144,12 @@ def test_oracle_ring_matches_the_window():
         orc.fill(tokens, ring, torch.tensor([length]), sinks)
         seen = orc.seen_pairs(length, window - 1, 0, sinks, None, None)[-1]
         assert sorted(ring[ring > 0].tolist()) == tokens[0, :length, 0, 0][seen].tolist()
+
+
+def test_a_ring_whose_size_passes_64_bits_is_refused():
+    lib = _cabi.load()
+    big = (1 << 63) - 1
+    assert lib.mvx_window_attention_step_workspace_bytes(0, 1, 1, 1, 8, big, big) == 0
+    for window, sinks in ((big, 1), (1, big), (big, big)):
+        assert lib.mvx_window_attention_step(SOME, SOME, SOME, 0, 1, 1, 1, 8, window, sinks, 1.0, SOME, SOME, SOME, SOME, None, 0,
+                                             None) == UNSUPPORTED

@@ -654,3 +654,150 @@ def test_gradients_of_rows_that_one_key_dominates(dtype):
         want = s @ other * scale
         bound = o @ other.abs() * scale
         within(a, want.transpose(0, 1)[None], (bound + u * (want.abs() + bound) + h).transpose(0, 1)[None], name)
+
+
+# ---- plans that the sizes above do not reach ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [
+    (4, 1700, 4, 2, 64, (16, 16), 1, (1700, 1, 1699, 33), False),   # float32: four waves walk a short window together
+    (1, 4500, 1, 1, 32, (20, 0), 33, None, False),                  # the far queries of the sinks in 32 chunks
+    (4, 1300, 6, 6, 32, (30, 0), 65, (1300, 700, 159, 0), True),    # chunks of 256
+    (1, 130, 1, 1, 128, (0, 129), 0, None, False),                  # looks ahead alone
+], ids=str)
+def test_window_attention_plans(dtype, case):
+    test_window_attention(dtype, case)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,slots,sinks", [(40, 1, 64, 2500, 3), (8, 2, 128, 5000, 16), (70, 2, 32, 90, 1),
+                                                           (4, 4, 96, 260, 0)])
+def test_window_attention_step_shares(dtype, heads, kv_heads, dim, slots, sinks):
+    """Long rings and many heads that share them.  Off by at most: u for the weights' rounding and u for the result's; twice
+    what float32 leaves of a score, (dim + 4) 2^-24 sum |q||k| scale; and of the sums over the slots, slots 2^-24 each."""
+    g = gen(heads + slots)
+    b, share, scale = 3, heads // kv_heads, dim ** -0.5
+    q = normal(g, (b, heads, dim), dtype)
+    k, v = normal(g, (b, kv_heads, dim), dtype), normal(g, (b, kv_heads, dim), dtype)
+    kc, vc = normal(g, (b, slots, kv_heads, dim), dtype), normal(g, (b, slots, kv_heads, dim), dtype)
+    lengths = torch.tensor([7 * slots, slots // 2, -3], device=DEV)
+    out = f64(temporal.window_attention_step(q, k, v, kc, vc, lengths, sinks))
+    assert (out[2] == 0).all()
+    u = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    for s, held in ((0, slots), (1, slots // 2 + 1)):
+        keys, values = (f64(c)[s, :held].repeat_interleave(share, 1).transpose(0, 1) for c in (kc, vc))
+        rows = f64(q)[s][:, None]
+        p = torch.softmax(rows @ keys.transpose(1, 2) * scale, -1)
+        score = (dim + 4) * 2.0 ** -24 * scale * (rows.abs() @ keys.abs().transpose(1, 2)).amax()
+        bound = (p @ values.abs())[:, 0] * (2 * u + 2 * score + 2 * slots * 2.0 ** -24)
+        within(out[s], (p @ values)[:, 0], bound, "stream %d" % s)
+
+
+def test_offsets_beyond_31_bits():
+    """The last rows of tensors of more than 2^31 values give what they give by themselves."""
+    g = gen(61)
+    n, tail = (1 << 22) + 1024, 1024  # tokens of 8 heads of 64
+    far = {name: torch.zeros(1, n, 8, 64, dtype=torch.bfloat16, device=DEV) for name in "qkvg"}
+    near = {name: normal(g, (1, tail, 8, 64), torch.bfloat16) for name in "qkvg"}
+    for name in "qkvg":
+        far[name][:, -tail:] = near[name]
+    out = {}
+    for side, t in (("far", far), ("near", near)):
+        leaves = [t[name].requires_grad_() for name in "qkv"]
+        y = temporal.window_attention(*leaves, (63, 0))
+        out[side] = [y.detach(), *torch.autograd.grad(y, leaves, t["g"])]
+    for a, c in zip(out["far"], out["near"]):
+        assert torch.equal(a[:, -tail + 128:], c[:, 128:])  # the first of the short sequence see fewer keys
+    del out
+    at = torch.arange(n, device=DEV)[:, None]
+    turned = temporal.rotate_positions(far["q"].detach(), far["k"].detach(), at, (32,))
+    alone = temporal.rotate_positions(near["q"].detach(), near["k"].detach(), at[-tail:], (32,))
+    assert all(torch.equal(a[:, -tail:], c) for a, c in zip(turned, alone))
+    del turned
+    x = far["q"].detach().view(-1, 512)
+    assert torch.equal(temporal.layer_norm(x)[-tail:], temporal.layer_norm(near["q"].detach().view(-1, 512)))
+    # a ring of 2 x 2.1 million slots, of which the last hold something
+    kc, vc = far["k"].detach().view(2, n // 2, 8, 64), far["v"].detach().view(2, n // 2, 8, 64)
+    slots = n // 2
+    q, k, v = (normal(g, (2, 8, 64), torch.bfloat16) for _ in range(3))
+    lengths = torch.tensor([-1, slots - 1], device=DEV)
+    step = temporal.window_attention_step(q, k, v, kc, vc, lengths, 4)
+    assert torch.equal(kc[1, -1], k[1]) and torch.equal(vc[1, -1], v[1]) and lengths.tolist() == [-1, slots]
+    keys, values = f64(kc[1, -tail:]).transpose(0, 1), f64(vc[1, -tail:]).transpose(0, 1)
+    weight = torch.exp(f64(q)[1][:, None] @ keys.transpose(1, 2) / 8)
+    total = weight.sum(-1) + (slots - tail)  # the other keys are zero: weights of 1, values of zero
+    want = (weight @ values)[:, 0] / total
+    # 2 u, and sums of 2^21 weights in float32: 32 at a time in a wave, at most 2^14 additions one after the other, 2^-24 each
+    within(step[1], want, (weight @ values.abs())[:, 0] / total * (2 ** -7 + 2 ** -9), "step")
+    temporal.window_cache_fill(near["k"].detach().expand(2, -1, -1, -1), near["v"].detach().expand(2, -1, -1, -1), kc, vc,
+                               torch.tensor([0, tail], device=DEV), slots - 10)
+    assert torch.equal(kc[1, :tail], near["k"][0]) and torch.equal(vc[1, :tail], near["v"][0])
+
+
+def test_two_graphs_and_eager_calls_in_turn():
+    """Workspaces belong to the graph that was captured with them."""
+    g = gen(62)
+
+    def work(seed, n, window, slots):
+        g = gen(seed)
+        q, k, v = (normal(g, (2, n, heads, 64), torch.bfloat16, True) for heads in (8, 2, 2))
+        up = normal(g, (2, n, 8, 64), torch.bfloat16)
+        kc, vc = normal(g, (2, slots, 2, 64), torch.bfloat16), normal(g, (2, slots, 2, 64), torch.bfloat16)
+        held = torch.full((2,), 3 * slots, device=DEV)
+
+        def run():
+            lengths = held.clone()
+            y = temporal.window_attention(q, k, v, window, 3)
+            grads = torch.autograd.grad(y, (q, k, v), up)
+            token = temporal.window_attention_step(q[:, 0].detach(), k[:, 0].detach(), v[:, 0].detach(), kc, vc, lengths, 3)
+            return [y.detach(), *grads, token]
+
+        return run
+
+    jobs = [work(1, 700, (50, 0), 900), work(2, 900, (70, 20), 700)]
+    want = [[t.clone() for t in job()] for job in jobs]
+    side = torch.cuda.Stream()
+    graphs, got = [], []
+    for job in jobs:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            job()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got.append(job())
+        graphs.append(graph)
+    for turn in range(6):
+        graphs[turn % 2].replay()
+        graphs[1 - turn % 2].replay()
+        eager = jobs[turn % 2]()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(eager, want[turn % 2]))
+        for one, c in zip(got, want):
+            assert all(torch.equal(a, e) for a, e in zip(one, c)), turn
+            for t in one:
+                t.zero_()
+    # and two streams at once
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        with torch.cuda.stream(side):
+            a = jobs[0]()
+        with torch.cuda.stream(other):
+            c = jobs[1]()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a, want[0])) and all(torch.equal(x, y) for x, y in zip(c, want[1]))
+
+
+@pytest.mark.parametrize("width", [1000, 9000])
+def test_layer_norm_of_16_bit_rows_with_float32_parameters(width):
+    g = gen(63)
+    x = normal(g, (37, width), torch.bfloat16, True)
+    w, b = normal(g, (width,), torch.float32, True, 0.3, 1.0), normal(g, (width,), torch.float32, True, 0.3)
+    up = normal(g, (37, width), torch.bfloat16)
+    got = torch.autograd.grad(temporal.layer_norm(x, w, b), (x, w, b), up)
+    assert [t.dtype for t in got] == [torch.bfloat16, torch.float32, torch.float32]
+    _, _, grads, bounds = orc.layer_norm(f64(x), f64(w), f64(b), 1e-5, torch.bfloat16, f64(up))
+    for name, a, c, e in zip(("dx", "dweight", "dbias"), got, grads, bounds):
+        within(a, c, e, name)
