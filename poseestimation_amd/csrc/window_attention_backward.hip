@@ -284,13 +284,13 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2
     for (int i = threadIdx.x; i < kSinkSums<DP>; i += 64 * kOwn) out[i] = shared.sums[i];
 }
 
-// Adds the chunks of one block of 32 sinks (blockIdx.y) into the first of them, in order.
+// Adds the chunks of one block of 32 sinks (blockIdx.x) into the first of them, in order.
 template <int DP>
 __global__ __launch_bounds__(256) void window_attention_sinks_join(AttentionShape a, int chunk, int chunks, float* __restrict__ partial) {
-    const int sink_blocks = (a.sinks + 31) / 32, block = blockIdx.y % sink_blocks;
-    const int64_t seq = blockIdx.y / sink_blocks / a.kv_heads;
+    const int sink_blocks = (a.sinks + 31) / 32, block = blockIdx.x % sink_blocks;
+    const int64_t seq = blockIdx.x / sink_blocks / a.kv_heads;
     const int length = seq_length(a, seq), left = length - window_end(a, block * 32 / kBlock * kBlock, length);
-    v4f* p = reinterpret_cast<v4f*>(partial + static_cast<int64_t>(blockIdx.y) * chunks * kSinkSums<DP>) + blockIdx.x * 256 + threadIdx.x;
+    v4f* p = reinterpret_cast<v4f*>(partial + static_cast<int64_t>(blockIdx.x) * chunks * kSinkSums<DP>) + blockIdx.y * 256 + threadIdx.x;
     const int filled = (left + chunk - 1) / chunk;
     if (filled <= 1) return;
     v4f sum = *p;
@@ -507,8 +507,7 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
     const TokenTensor ot = {out, n_tokens * row, row, dim};
     const int blocks = static_cast<int>((n_tokens + kBlock - 1) / kBlock);
     const FarPlan f = far_plan(n_seqs * kv_heads, n_tokens, left, sinks);
-    MVX_REQUIRE(n_seqs <= (1 << 23) / blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23) &&
-                    n_seqs * kv_heads * f.sink_blocks <= 65535,
+    MVX_REQUIRE(n_seqs <= (1 << 23) / blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23),
                 MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch", name);
     float* delta = static_cast<float*>(workspace);
     float* partial = delta + padded_rows(n_seqs * heads * n_tokens);
@@ -525,7 +524,7 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
                 hipLaunchKernelGGL(sinks_kernel, dim3(sinks_of_all * f.chunks), dim3(64 * sink_waves), 0, st, qt, kt, vt, gt, s, f.chunk,
                                    f.chunks, lse, d, partial);
             if (f.chunks > 1)
-                hipLaunchKernelGGL(join_kernel, dim3(padded_dim(dim) * 64 / 4 / 256, sinks_of_all), dim3(256), 0, st, s, f.chunk, f.chunks,
+                hipLaunchKernelGGL(join_kernel, dim3(sinks_of_all, padded_dim(dim) * 64 / 4 / 256), dim3(256), 0, st, s, f.chunk, f.chunks,
                                    partial);
             hipLaunchKernelGGL(dkv_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
                                vt, gt, s, scale, blocks, f.chunks, lse, d, partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));

@@ -801,3 +801,16 @@ def test_layer_norm_of_16_bit_rows_with_float32_parameters(width):
     _, _, grads, bounds = orc.layer_norm(f64(x), f64(w), f64(b), 1e-5, torch.bfloat16, f64(up))
     for name, a, c, e in zip(("dx", "dweight", "dbias"), got, grads, bounds):
         within(a, c, e, name)
+
+
+def test_gradients_of_sinks_of_very_many_sequences():
+    b, n, heads, dim, dtype = 4200, 700, 16, 8, torch.float16
+    torch.manual_seed(64)
+    q, k, v, up = (torch.randn(b, n, heads, dim, device=DEV, dtype=dtype) for _ in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(temporal.window_attention(*leaves, (0, 0), 2), leaves, up)
+    for s in (0, b - 1):
+        one = slice(s, s + 1)
+        _, _, grads, bounds = orc.attention(f64(q[one]), f64(k[one]), f64(v[one]), (0, 0), 2, dtype, grad=f64(up[one]))
+        for name, a, c, e in zip(("dq", "dk", "dv"), got, grads, bounds):
+            within(a[one], c, e, "%s of sequence %d" % (name, s))
