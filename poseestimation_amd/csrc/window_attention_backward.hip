@@ -23,7 +23,7 @@ namespace mvx {
 
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlock = 32 * kWaves;
+constexpr int kBlock = 128;  // queries and keys of a workgroup of four waves; where the far queries of sinks begin
 
 // In the place of a query's delta: it sees a single key.  A NaN of its own, which no arithmetic makes.
 constexpr unsigned kAlone = 0x7fe5a10eu;
@@ -32,13 +32,13 @@ __device__ __forceinline__ bool is_alone(float delta) { return __builtin_bit_cas
 // The lowest n bits.
 __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
+template <typename T, int DP, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 : 128) ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
                                                                 const T* __restrict__ rest, TokenTensor g, AttentionShape a, float scale, int q_blocks,
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
                                                                 T* __restrict__ dq) {
     using Tl = Tiles<T, DP>;
-    constexpr int kTile = kTileRows<T>;
+    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kWaves == 1 ? 32 : kTileRows<T>;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kTile * Tl::LD];
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     const int head = kv_head * share + in_group;
     const int half = lane_id() >> 5, wave = wave_id();
     const int length = seq_length(a, seq);
-    const int q0 = block * kBlock, w0 = q0 + wave * 32, mine = w0 + (lane_id() & 31);
+    const int q0 = block * kMine, w0 = q0 + wave * 32, mine = w0 + (lane_id() & 31);
 
     const T* kb = static_cast<const T*>(k.p) + seq * k.seq + kv_head * k.head;
     const T* vb = static_cast<const T*>(v.p) + seq * v.seq + kv_head * v.head;
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void windo
     if (live) my_lse = lse[at_row];
 
     const int hi = live ? min(mine + a.right, length - 1) : -1, lo = mine - a.left;
-    const KeyTiles tiles = key_tiles(a, q0, kBlock, length, kTile);
+    const KeyTiles tiles = key_tiles(a, q0, kMine, length, kTile);
     // Counted ahead of the products, which have no registers left (counting along with them took 3 to 6 % more time).
     int n_seen = max(0, hi + 1 - max(lo, 0)) + max(0, min(min(a.sinks, hi + 1), lo));
     if (a.visible != nullptr) {
@@ -299,15 +299,15 @@ __global__ __launch_bounds__(256) void window_attention_sinks_join(AttentionShap
     *p = sum;
 }
 
-// Keys [k0, k0 + 128) of one key/value head and the queries of the block's window.
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
+// Keys [k0, k0 + 32 kWaves) of one key/value head and the queries of the block's window.
+template <typename T, int DP, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? (DP <= (sizeof(T) == 4 ? 64 : 96)) + 1 : (sizeof(T) * DP <= 128) + 1) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
                                                                  AttentionShape a, float scale, int k_blocks, int chunks,
                                                                  const float* __restrict__ lse, const float* __restrict__ delta,
                                                                  float* __restrict__ partial,
                                                                  T* __restrict__ dk, T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
-    constexpr int kTile = kTileRows<T>;
+    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kWaves == 1 ? 32 : kTileRows<T>;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell q_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell g_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse, delta
@@ -319,8 +319,9 @@ __global__ __launch_bounds__(kThreads, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1)
     const int share = a.heads / a.kv_heads;
     const int half = lane_id() >> 5, wave = wave_id();
     const int length = seq_length(a, seq);
-    const int k0 = block * kBlock, w0 = k0 + wave * 32, mine = w0 + (lane_id() & 31);
-    const int begin = max(0, k0 - a.right), end = window_end(a, k0, length);
+    const int k0 = block * kMine, w0 = k0 + wave * 32, mine = w0 + (lane_id() & 31);
+    const int begin = max(0, k0 - a.right);
+    const int end = k0 < a.sinks ? window_end(a, k0 / kBlock * kBlock, length) : min(length, k0 + kMine + a.left);
     const int per_head = begin < end && k0 < length ? (end - begin + kTile - 1) / kTile : 0, tiles = per_head * share;
 
     const bool kept = mine < length && (a.visible == nullptr || a.visible[seq * a.n_tokens + mine] != 0);
@@ -457,6 +458,15 @@ FarPlan far_plan(int64_t rows, int64_t n_tokens, int64_t left, int64_t sinks) { 
     f.chunks = static_cast<int>((far + chunk - 1) / chunk);
     return f;
 }
+// Waves of a workgroup of the first and the last kernel, each with 32 queries or keys.  Four share their tiles; where that leaves
+// CUs without work, two take their place if the window is short (4 x 2000 x 2 x 32 float32, 127 keys: 128 workgroups of four 41 us,
+// twice as many of two 34 us; 257 tokens x 4 heads x 64, 33 keys: 24 -> 18 us) or the heads are so long that four waves keep few of
+// their registers (2048 x 4 x 128 bfloat16, all keys: 105 -> 74 us).  Long windows of shorter heads gain from the sharing
+// (2048 x 4 x 64 float32, all keys: 147 and 167 us).
+int waves_of_block(int64_t rows, const AttentionShape& s) {  // rows: sequences times heads
+    const bool idle = rows * ((s.n_tokens + kBlock - 1) / kBlock) < 256;
+    return idle && (static_cast<int64_t>(s.left) + s.right < 256 || s.dim > 64) ? 2 : 4;
+}
 int padded_dim(int dim) { return (dim + 31) / 32 * 32; }
 
 }  // namespace
@@ -505,20 +515,21 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
                 name, need, workspace_bytes);
     const int64_t row = static_cast<int64_t>(heads) * dim;
     const TokenTensor ot = {out, n_tokens * row, row, dim};
-    const int blocks = static_cast<int>((n_tokens + kBlock - 1) / kBlock);
+    const int q_waves = waves_of_block(n_seqs * heads, s), q_blocks = (s.n_tokens + 32 * q_waves - 1) / (32 * q_waves);
+    const int k_waves = waves_of_block(n_seqs * kv_heads, s), k_blocks = (s.n_tokens + 32 * k_waves - 1) / (32 * k_waves);
     const FarPlan f = far_plan(n_seqs * kv_heads, n_tokens, left, sinks);
-    MVX_REQUIRE(n_seqs <= (1 << 23) / blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23),
+    MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads && n_seqs * kv_heads * f.sink_blocks * f.chunks <= (1 << 23),
                 MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch", name);
     float* delta = static_cast<float*>(workspace);
     float* partial = delta + padded_rows(n_seqs * heads * n_tokens);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
+        const float *d = delta, *lse = static_cast<const float*>(saved);
+        const T* rest = reinterpret_cast<const T*>(lse + padded_rows(n_seqs * heads * n_tokens));
         const auto launch = [&](auto dq_kernel, auto sinks_kernel, int sink_waves, auto join_kernel, auto dkv_kernel) {
-            const float *d = delta, *lse = static_cast<const float*>(saved);
-            const T* rest = reinterpret_cast<const T*>(lse + padded_rows(n_seqs * heads * n_tokens));
-            hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * blocks)), dim3(kThreads), 0, st, qt, kt, vt,
-                               ot, rest, gt, s, scale, blocks, lse, delta, static_cast<T*>(grad_q));
+            hipLaunchKernelGGL(dq_kernel, dim3(static_cast<unsigned>(n_seqs * heads * q_blocks)), dim3(64 * q_waves), 0, st, qt, kt, vt,
+                               ot, rest, gt, s, scale, q_blocks, lse, delta, static_cast<T*>(grad_q));
             const unsigned sinks_of_all = static_cast<unsigned>(n_seqs * kv_heads * f.sink_blocks);
             if (f.chunks > 0)
                 hipLaunchKernelGGL(sinks_kernel, dim3(sinks_of_all * f.chunks), dim3(64 * sink_waves), 0, st, qt, kt, vt, gt, s, f.chunk,
@@ -526,21 +537,22 @@ extern "C" int mvx_window_attention_backward(const void* q, const int64_t* q_str
             if (f.chunks > 1)
                 hipLaunchKernelGGL(join_kernel, dim3(sinks_of_all, padded_dim(dim) * 64 / 4 / 256), dim3(256), 0, st, s, f.chunk, f.chunks,
                                    partial);
-            hipLaunchKernelGGL(dkv_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * blocks)), dim3(kThreads), 0, st, qt, kt,
-                               vt, gt, s, scale, blocks, f.chunks, lse, d, partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+            hipLaunchKernelGGL(dkv_kernel, dim3(static_cast<unsigned>(n_seqs * kv_heads * k_blocks)), dim3(64 * k_waves), 0, st, qt, kt,
+                               vt, gt, s, scale, k_blocks, f.chunks, lse, d, partial, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
         };
+#define MVX_LAUNCH(DP)                                                                                                        \
+    launch(q_waves == 2 ? window_attention_dq<T, DP, 2> : window_attention_dq<T, DP, 4>, window_attention_sinks<T, DP>,      \
+           kSinkWaves<T, DP>, window_attention_sinks_join<DP>,                                                                \
+           k_waves == 2 ? window_attention_dkv<T, DP, 2> : window_attention_dkv<T, DP, 4>)
         if (dim <= 32)
-            launch(window_attention_dq<T, 32>, window_attention_sinks<T, 32>, kSinkWaves<T, 32>, window_attention_sinks_join<32>,
-                   window_attention_dkv<T, 32>);
+            MVX_LAUNCH(32);
         else if (dim <= 64)
-            launch(window_attention_dq<T, 64>, window_attention_sinks<T, 64>, kSinkWaves<T, 64>, window_attention_sinks_join<64>,
-                   window_attention_dkv<T, 64>);
+            MVX_LAUNCH(64);
         else if (dim <= 96)
-            launch(window_attention_dq<T, 96>, window_attention_sinks<T, 96>, kSinkWaves<T, 96>, window_attention_sinks_join<96>,
-                   window_attention_dkv<T, 96>);
+            MVX_LAUNCH(96);
         else
-            launch(window_attention_dq<T, 128>, window_attention_sinks<T, 128>, kSinkWaves<T, 128>, window_attention_sinks_join<128>,
-                   window_attention_dkv<T, 128>);
+            MVX_LAUNCH(128);
+#undef MVX_LAUNCH
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });

@@ -814,3 +814,14 @@ def test_gradients_of_sinks_of_very_many_sequences():
         _, _, grads, bounds = orc.attention(f64(q[one]), f64(k[one]), f64(v[one]), (0, 0), 2, dtype, grad=f64(up[one]))
         for name, a, c, e in zip(("dq", "dk", "dv"), got, grads, bounds):
             within(a[one], c, e, "%s of sequence %d" % (name, s))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [
+    (1, 300, 2, 1, 128, (None, 0), 3, None, False),
+    (1, 600, 4, 4, 96, (100, 20), 40, (555,), True),
+    (16, 500, 4, 1, 32, (50, 0), 2, None, True),     # pairs of waves for the keys, four waves for the queries
+    (4, 1800, 8, 8, 16, (255, 0), 1, None, False),   # four waves for both
+], ids=str)
+def test_window_attention_gradients_by_pairs_of_waves(dtype, case):
+    test_window_attention(dtype, case)
