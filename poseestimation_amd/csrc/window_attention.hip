@@ -4,14 +4,23 @@
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i) over the seen keys; a row that sees none is zero
 //
 // A wave takes 32 queries of one head; a workgroup of 4 waves (or of one, for short windows) walks the tiles of 64 (32) keys
-// that any of its queries sees: first those of the sinks, then the window.  Scores come out transposed (keys in registers, queries in lanes), so the
-// softmax of a query runs inside a lane and its partner 32 lanes on, with a running maximum and sum, and the weighted sum of
-// the values takes the scores where they lie.  A tile is held in LDS for all waves and the next one travels from memory
-// meanwhile; tiles that every query sees whole skip the mask, and a wave skips a tile that none of its queries sees.
+// that any of its queries sees: first those of the sinks, then the window.  Scores come out transposed (keys in registers,
+// queries in lanes), so the softmax of a query runs inside a lane and its partner 32 lanes on, with a running maximum and sum,
+// and the weighted sum of the values takes the scores where they lie.  A tile is held in LDS for all waves and the next one
+// travels from memory meanwhile; tiles that every query sees whole skip the mask, and a wave skips a tile that none of its
+// queries sees.
 // Scores and sums are float32; the weights (at most 2^kSlack) are rounded to the element type for the second product.  The sum
 // that divides the result is that of the rounded weights: the result is a mean of the values whose weights are off by relative
 // errors alone, so a row that one key dominates is as exact as that key's value, which the backward's differences need.  What
 // the backward takes the weights from, the logarithm of the sum, is that of the weights before rounding.
+//
+// Bound by the matrix and vector units taking turns: the softmax of a block takes about as long as its products, and two waves
+// per SIMD, all that the registers hold, do not hide one behind the other (counters of 8192 tokens x 16 heads of 128, 1040 keys:
+// matrix units busy 31 % of the time, vector units 39 %).  bfloat16, each with the flops of the pairs that are seen: that prompt
+// 97 us (670 Tflop/s), all keys of 2 x 4096 x 16: heads of 64 225 us (610), of 128 330 us (830); 4 x 4096 x 8 x 64 with 256 keys
+// and 4 sinks 36 us (240; blocks cut by the window's edges and the sinks' add a third to the products, and a workgroup's eight
+// tiles leave its first loads exposed).  A large product reaches 1100.  float32 in its three parts: 4 x 4096 x 8 x 64, 1024 keys,
+// 206 us.
 #include "attention_tiles.h"
 
 namespace mvx {
@@ -26,6 +35,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
     TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest) {
     using Tl = Tiles<T, DP>;
     constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = kWaves == 1 ? 32 : kTileRows<T>;  // queries of the workgroup, keys of a tile
+    // Copies of the loop over blocks of 32 keys: of longer heads two need more registers than two waves per SIMD have (4 x 4096 x
+    // 8 x 64 bfloat16, 255 keys: 37 us with one, 35 with two).
+    constexpr int kBlocks = DP <= 64 ? kBK / 32 : 1;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kBK * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kBK * Tl::LD];
     // heads that share keys, then blocks of queries, are neighbours on one XCD
@@ -88,7 +100,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
         if (t + 2 < tiles.count) fetch(t + 2);
         const int k0 = tiles.key0(t, kBK);
         const typename Tl::Cell *kt = k_tile[t & 1], *vt = v_tile[t & 1];
-#pragma unroll 1  // two copies need more registers than two waves per SIMD have
+#pragma unroll kBlocks
         for (int b = 0; b < kBK; b += 32) {
             if (!sees_any(a, w0, k0 + b, 32, length)) continue;
             typename Tl::Pool pool;
