@@ -29,6 +29,11 @@ constexpr int kBlock = 128;  // queries and keys of a workgroup of four waves; w
 constexpr unsigned kAlone = 0x7fe5a10eu;
 __device__ __forceinline__ bool is_alone(float delta) { return __builtin_bit_cast(unsigned, delta) == kAlone; }
 
+// Copies of a tile's loop over its blocks of 32 rows: of longer heads two need more registers than two waves per SIMD have
+// (4 x 4096 x 8 x 64 bfloat16, 255 keys: dq 50 us with one copy, 47 with two; dk and dv 49 and 48).
+template <int DP, int TILE>
+constexpr int kBlocksOf = DP <= 64 ? TILE / 32 : 1;
+
 // The lowest n bits.
 __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 
@@ -38,7 +43,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 :
                                                                 const float* __restrict__ lse, float* __restrict__ delta,
                                                                 T* __restrict__ dq) {
     using Tl = Tiles<T, DP>;
-    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kWaves == 1 ? 32 : kTileRows<T>;
+    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kBlocksOf<DP, kTile>;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kTile * Tl::LD];
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -130,7 +135,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 :
         const int at = k0 + 4 * half;
         const int hi_r = hi - at, lo_r = lo - at, sink_r = a.sinks - at;
         const uint64_t bits = keep >> (4 * half);
-#pragma unroll 1  // two copies need more registers than two waves per SIMD have
+#pragma unroll kBlocks
         for (int b = 0; b < kTile / 32; ++b) {
             if (!sees_any(a, w0, k0 + 32 * b, 32, length)) continue;
             const bool whole = static_cast<unsigned>(keep >> (32 * b)) == ~0u && sees_all(a, w0, k0 + 32 * b, 32, length);
@@ -307,7 +312,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? (DP <= (sizeof(T) == 4 ?
                                                                  float* __restrict__ partial,
                                                                  T* __restrict__ dk, T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
-    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kWaves == 1 ? 32 : kTileRows<T>;
+    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kBlocksOf<DP, kTile>;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell q_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell g_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse, delta
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? (DP <= (sizeof(T) == 4 ?
         if (w0 >= length) continue;
         const typename Tl::Cell *qt = q_tile[t & 1], *gt = g_tile[t & 1];
         const int at = i0 + 4 * half, lo_r = lo - at, hi_r = min(hi, end - 1) - at;
-#pragma unroll 1  // two copies need more registers than two waves per SIMD have
+#pragma unroll kBlocks
         for (int b = 0; b < kTile / 32; ++b) {
             const int r0 = i0 + 32 * b;  // the block's first query
             if (r0 >= end || r0 + 32 <= w0 - a.right || r0 > wave_last) continue;
