@@ -11,8 +11,8 @@
 // The backward keeps dw and db of the lane's columns in registers over all rows its workgroup visits, loads the next row while
 // it works on one, and writes one row of partial sums per workgroup; a second launch adds those up in a fixed order (no atomics:
 // the result is the same in every run).
-// 65536 x 1024 bfloat16: forward 53 us (5.1 TB/s, a large copy's rate), backward 85 us (4.7 TB/s); 32768 x 1024 float32: 44 and
-// 80 us.
+// 65536 x 1024 bfloat16: forward 50 us (5.4 TB/s, a large copy's rate is 5.0), backward 86 us (4.7 TB/s); 32768 x 1024 float32:
+// 49 and 82 us.
 #include "element.h"
 
 namespace mvx {

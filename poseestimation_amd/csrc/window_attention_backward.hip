@@ -17,6 +17,11 @@
 // A query that sees a single key weighs it with 1 whatever its score: dp - delta is zero there, but rounding would leave noise,
 // which is all there is where every query sees one key.  The first kernel counts the keys a query sees, gives such a query no
 // gradient, and leaves a mark in the place of its delta.
+//
+// bfloat16, 4 x 4096 x 8 x 64 with 256 keys and 4 sinks: dq 47 us, far queries 12, their sums 5, dk and dv 48; what these have to
+// read and write takes 23, 7, 1 and 20 us at a large copy's rate, the rest is the latency of a few tiles per workgroup.  All keys
+// of 2 x 4096 x 8 x 64: 290 us together (590 Tflop/s of the five products that are counted; two more are computed), of
+// 4096 x 16 x 128, causal: 540 us (320): one wave per SIMD for dk and dv, whose sums alone take half of the registers.
 #include "attention_tiles.h"
 
 namespace mvx {

