@@ -998,8 +998,8 @@ def main():
         sys.exit(2)
     visible = torch.cuda.device_count()
     if not rehearsal and visible < (local_rank + 1 if launch.in_launched_rank() else 1):
-        if rank == 0:
-            print("bench.py: --gpus %d but %d GPU(s) visible" % (args.gpus, visible), file=sys.stderr)
+        # every rank says so: the first to exit has the others stopped, maybe before rank 0 gets here
+        print("bench.py: --gpus %d but %d GPU(s) visible" % (args.gpus, visible), file=sys.stderr)
         sys.exit(2)
     dev = torch.device("cuda", 0 if rehearsal else local_rank)
     torch.cuda.set_device(dev)
