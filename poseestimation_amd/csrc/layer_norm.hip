@@ -8,11 +8,12 @@
 // there and written once.  A row is held by one wave (up to 4 vectors of 16 bytes per lane), by 256 or by 1024 threads; its
 // vectors are loaded at element alignment, and the last one is moved back to end with the row (its first elements then
 // repeat another lane's and are left out of the sums), so odd widths run at the same rate as even ones.
-// The backward keeps dw and db of the lane's columns in registers over all rows its workgroup visits, loads the next row while
-// it works on one, and writes one row of partial sums per workgroup; a second launch adds those up in a fixed order (no atomics:
+// Both directions load the next row while they work on one; the forward keeps the weights of the lane's columns in registers.
+// The backward keeps dw and db of the lane's columns there, over all rows its workgroup visits, and writes one row of partial sums
+// per workgroup; a second launch adds those up in a fixed order (no atomics:
 // the result is the same in every run).
-// 65536 x 1024 bfloat16: forward 50 us (5.4 TB/s, a large copy's rate is 5.0), backward 86 us (4.7 TB/s); 32768 x 1024 float32:
-// 49 and 82 us.
+// 65536 x 1024 bfloat16: forward 43 us (6.2 TB/s; a large copy runs at 5.0), backward 85 us (4.7 TB/s); 32768 x 1024 float32: 42
+// and 82 us.
 #include "element.h"
 
 namespace mvx {
@@ -98,9 +99,21 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows(const T* __restrict__ x
 #pragma unroll
     for (int n = 0; n < NV; ++n) place_vec(t + n * ROW_T, VEC, width, &start[n], &fresh[n]);
     const float inv_width = 1.0f / static_cast<float>(width);
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * (BLOCK / ROW_T) + threadIdx.x / ROW_T; row < rows; row += stride) {
-        RowVecs<T, NV> xv;
-        xv.load(x + row * width, start, fresh);
+    int64_t row = static_cast<int64_t>(blockIdx.x) * (BLOCK / ROW_T) + threadIdx.x / ROW_T;
+    float w[NV][VEC], b[NV][VEC];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[n][e] = 1.0f, b[n][e] = 0.0f;
+        if (fresh[n] >= VEC) continue;
+        if (weight != nullptr) load_param<T>(weight, param_f32, start[n], w[n]);
+        if (bias != nullptr) load_param<T>(bias, param_f32, start[n], b[n]);
+    }
+    RowVecs<T, NV> x_next;
+    if (row < rows) x_next.load(x + row * width, start, fresh);
+    for (; row < rows; row += stride) {
+        RowVecs<T, NV> xv = x_next;
+        if (row + stride < rows) x_next.load(x + (row + stride) * width, start, fresh);  // travels while this row is worked on
         float v[NV][VEC];
 #pragma unroll
         for (int n = 0; n < NV; ++n)
@@ -131,14 +144,9 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows(const T* __restrict__ x
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             if (fresh[n] >= VEC) continue;
-            float w[VEC], b[VEC], out[VEC];
-            if (weight != nullptr) load_param<T>(weight, param_f32, start[n], w);
-            if (bias != nullptr) load_param<T>(bias, param_f32, start[n], b);
+            float out[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float h = v[n][e] * rstd;
-                out[e] = fmaf(h, weight != nullptr ? w[e] : 1.0f, bias != nullptr ? b[e] : 0.0f);
-            }
+            for (int e = 0; e < VEC; ++e) out[e] = fmaf(v[n][e] * rstd, w[n][e], b[n][e]);
             store_vec<T>(yr + start[n], out);
         }
     }
@@ -395,8 +403,13 @@ int backward_groups(int64_t rows, int64_t width, int vec) {
     return static_cast<int>(need < most ? (need > 0 ? need : 1) : most);
 }
 
-// Workgroups of a grid-stride kernel: work-items of a launch stay below 2^32.
-unsigned capped(int64_t blocks) { return static_cast<unsigned>(blocks < (1 << 21) ? blocks : (1 << 21)); }
+// Workgroups of the forward: few enough that each takes several rows, with its weights in registers and the next row on its way
+// (65536 x 1024 bfloat16: 43 us with 1024 of four rows, 47 with 8192, 49 with one row per wave and nothing in flight; 8192 x 8192
+// float16: 47 us with 2048 of one row, 50 with 1024, 54 with one row each).
+unsigned forward_groups(int64_t rows, int block, int row_t) {
+    const int64_t groups = (rows + block / row_t - 1) / (block / row_t), most = row_t == 64 ? 1024 : 2048;
+    return static_cast<unsigned>(groups < most ? groups : most);
+}
 
 // Dynamic LDS of the backward: the weight, and where rows share a workgroup the columns' sums in the same place.
 size_t norm_lds(int64_t width, int row_t, int nv, int vec, bool sums) {
@@ -433,8 +446,7 @@ extern "C" int mvx_layer_norm(const void* x, const void* weight, const void* bia
         const int w = static_cast<int>(width);
 #define MVX_NORM(ROW_T, BLOCK, NV)                                                                                             \
     if (p.row_t == ROW_T && p.nv == NV)                                                                                        \
-        hipLaunchKernelGGL((layer_norm_rows<T, ROW_T, BLOCK, NV>), dim3(capped((rows + BLOCK / ROW_T - 1) / (BLOCK / ROW_T))), \
-                           dim3(BLOCK), 0, st, xt, weight, bias, param_f32, rows, w, eps, yt, stats)
+        hipLaunchKernelGGL((layer_norm_rows<T, ROW_T, BLOCK, NV>), dim3(forward_groups(rows, BLOCK, ROW_T)), dim3(BLOCK), 0, st, xt, weight, bias, param_f32, rows, w, eps, yt, stats)
         MVX_NORM(64, 256, 1);
         MVX_NORM(64, 256, 2);
         MVX_NORM(64, 256, 4);
