@@ -7,8 +7,8 @@
 // The backward is the rotation by the opposite angle.  Angles are formed in float64 as revolutions and reduced there
 // (position 10^6 at frequency 1 would keep four digits in float32); cos and sin of the reduced angle are float32.
 //
-// Bound by memory: q and k are read once and written once in one launch (8 x 4608 tokens x 20 heads of 128 bfloat16: 72 us,
-// 5.2 TB/s, a large copy's rate).  A workgroup takes a few tokens, computes their cos / sin once into LDS and applies them to
+// Bound by memory: q and k are read once and written once in one launch (8 x 4608 tokens x 20 heads of 128 bfloat16: 68 us,
+// 5.5 TB/s; a large copy runs at 5.0).  A workgroup takes a few tokens, computes their cos / sin once into LDS and applies them to
 // all heads of q and k, 16 bytes per access.  Vectors are placed at element alignment with the last one of a stretch moved back to its end (its first values are then written twice, with the same
 // result), so any number of pairs runs at the vector rate; stretches shorter than a vector go element by element.
 #include <math.h>
@@ -193,9 +193,10 @@ extern "C" int mvx_rotate_positions(const void* q, const int64_t* q_strides, int
         const int units = (span + VEC - 1) / VEC + (dim - 2 * p + VEC - 1) / VEC;
         const int64_t per_token = static_cast<int64_t>(units) * (q_heads + k_heads);
         MVX_REQUIRE(per_token <= (1 << 24), MVX_ERR_UNSUPPORTED, "%s: too many heads", name);
-        // tokens of a workgroup: about four vectors of work per thread, at most 16 KB of cos and sin; a short call takes
-        // one token per workgroup, so that its few tokens run side by side
-        int64_t per_block = 1024 / per_token;
+        // Tokens of a workgroup: about 16 KB of values (two vectors per unit of halves, one of neighbours; 8 x 4608 tokens x 20
+        // heads of 128 bfloat16: halves 68 us with 512 units, 73 with 1024; neighbours 87 and 71), at most 16 KB of cos and sin.
+        // A short call takes one token per workgroup, so that its few tokens run side by side.
+        int64_t per_block = (adjacent_pairs ? 1024 : 512) / per_token;
         if (per_block > 2048 / p) per_block = 2048 / p;
         if (per_block < 1 || rows < 1024) per_block = 1;
         const int64_t blocks = (rows + per_block - 1) / per_block;
