@@ -3,12 +3,12 @@
 //   key j is seen by query i iff j <= i + right and (j >= i - left or j < sinks), j < length, visible[j]
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i) over the seen keys; a row that sees none is zero
 //
-// A wave takes 32 queries of one head; a workgroup of 4 waves (or of one, for short windows) walks the tiles of 64 (32) keys
-// that any of its queries sees: first those of the sinks, then the window.  Scores come out transposed (keys in registers,
-// queries in lanes), so the softmax of a query runs inside a lane and its partner 32 lanes on, with a running maximum and sum,
-// and the weighted sum of the values takes the scores where they lie.  A tile is held in LDS for all waves and the next one
-// travels from memory meanwhile; tiles that every query sees whole skip the mask, and a wave skips a tile that none of its
-// queries sees.
+// A wave takes 32 queries of one head; a workgroup of 4 waves (or of one, for short windows, whose keys two waves may share) walks
+// the tiles of 64 (32) keys that any of its queries sees: first those of the sinks, then the window.  Scores come out
+// transposed (keys in registers, queries in lanes), so the softmax of a query runs inside a lane and its partner 32 lanes on,
+// with a running maximum and sum, and the weighted sum of the values takes the scores where they lie.  A tile is held in LDS
+// for all waves and the next one travels from memory meanwhile; tiles that every query sees whole skip the mask, and a wave
+// skips a tile that none of its queries sees.
 // Scores and sums are float32; the weights (at most 2^kSlack) are rounded to the element type for the second product.  The sum
 // that divides the result is that of the rounded weights: the result is a mean of the values whose weights are off by relative
 // errors alone, so a row that one key dominates is as exact as that key's value, which the backward's differences need.  What
@@ -30,16 +30,18 @@ namespace {
 constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2^15
 
 // The registers are cut for two waves per SIMD where they suffice: with one, a long prompt of heads of 128 took 1.8 times as long.
-template <typename T, int DP, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
+// kWaves: waves with queries of their own, which share tiles; kSplit: waves that share the queries of one, each with every
+// kSplit-th tile, kept to itself.
+template <typename T, int DP, int kWaves, int kSplit>
+__global__ __launch_bounds__(64 * kWaves * kSplit, kWaves > 1 && sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
     TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest) {
     using Tl = Tiles<T, DP>;
     constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = kWaves == 1 ? 32 : kTileRows<T>;  // queries of the workgroup, keys of a tile
     // Copies of the loop over blocks of 32 keys: of longer heads two need more registers than two waves per SIMD have (4 x 4096 x
     // 8 x 64 bfloat16, 255 keys: 37 us with one, 35 with two).
     constexpr int kBlocks = DP <= 64 ? kBK / 32 : 1;
-    __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kBK * Tl::LD];
-    __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kBK * Tl::LD];
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[kSplit][2][kBK * Tl::LD];
+    __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[kSplit][2][kBK * Tl::LD];
     // heads that share keys, then blocks of queries, are neighbours on one XCD
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int share = a.heads / a.kv_heads;
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
     const int kv_head = id % a.kv_heads;
     const int64_t seq = id / a.kv_heads;
     const int head = kv_head * share + in_group;
-    const int half = lane_id() >> 5, wave = wave_id();
+    const int half = lane_id() >> 5, wave = kSplit == 1 ? wave_id() : 0, part = kSplit == 1 ? 0 : wave_id();
     const int length = seq_length(a, seq);
     const int q0 = block * kBQ, w0 = q0 + wave * 32;  // the workgroup's and the wave's first query
 
@@ -67,12 +69,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
     float top = -kInf, sum = 0.0f, divisor = 0.0f;
 
     const KeyTiles tiles = key_tiles(a, q0, kBQ, length, kBK);
+    const int n_tiles = (tiles.count - part + kSplit - 1) / kSplit;  // of this wave: part, part + kSplit, ...
     TileInFlight<T, DP, kBK, 64 * kWaves> k_next, v_next;
     k_next.place(k.token, a.dim);
     v_next.place(v.token, a.dim);
     bool kept_next = false;
     const auto fetch = [&](int t) {
-        const int k0 = tiles.key0(t, kBK);
+        const int k0 = tiles.key0(part + t * kSplit, kBK);
         k_next.load(kb, k.token, k0, length);
         v_next.load(vb, v.token, k0, length);
         kept_next = token_kept(a, seq, k0, length);
@@ -83,23 +86,27 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
             k_next.hide(keep);
             v_next.hide(keep);
         }
-        k_next.store(k_tile[t & 1]);
-        v_next.store(v_tile[t & 1]);
+        k_next.store(k_tile[part][t & 1]);
+        v_next.store(v_tile[part][t & 1]);
         return keep;
     };
     uint64_t keep = 0, keep_next = 0;
-    if (tiles.count > 0) {
+    if (n_tiles > 0) {
         fetch(0);
         keep_next = put(0);
     }
-    if (tiles.count > 1) fetch(1);
-    for (int t = 0; t < tiles.count; ++t) {
+    if (n_tiles > 1) fetch(1);
+    for (int t = 0; t < n_tiles; ++t) {
         keep = keep_next;
-        __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
-        if (t + 1 < tiles.count) keep_next = put(t + 1);
-        if (t + 2 < tiles.count) fetch(t + 2);
-        const int k0 = tiles.key0(t, kBK);
-        const typename Tl::Cell *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+        // tile t is in LDS, and nobody reads tile t - 1 any more
+        if constexpr (kSplit == 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (t + 1 < n_tiles) keep_next = put(t + 1);
+        if (t + 2 < n_tiles) fetch(t + 2);
+        const int k0 = tiles.key0(part + t * kSplit, kBK);
+        const typename Tl::Cell *kt = k_tile[part][t & 1], *vt = v_tile[part][t & 1];
 #pragma unroll kBlocks
         for (int b = 0; b < kBK; b += 32) {
             if (!sees_any(a, w0, k0 + b, 32, length)) continue;
@@ -150,6 +157,33 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 1 && sizeof(T) * DP <= 256 ? 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += s[i];
             }
+        }
+    }
+    if constexpr (kSplit > 1) {  // the waves' lanes hold the same queries: the first adds up what the others leave, in order
+        __shared__ float left_by[kSplit - 1][DT * 16 + 3][64];
+        if (part > 0) {
+            float(*mine)[64] = left_by[part - 1];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine[dt * 16 + i][lane_id()] = acc[dt][i];
+            mine[DT * 16][lane_id()] = top;
+            mine[DT * 16 + 1][lane_id()] = sum;
+            mine[DT * 16 + 2][lane_id()] = divisor;
+        }
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int n = 0; n < kSplit - 1; ++n) {
+            const float top2 = left_by[n][DT * 16][lane_id()], next = fmaxf(top, top2), ref = next == -kInf ? 0.0f : next;
+            const float f = __builtin_amdgcn_exp2f(top - ref), f2 = __builtin_amdgcn_exp2f(top2 - ref);
+            top = next;
+            sum = sum * f + left_by[n][DT * 16 + 1][lane_id()] * f2;
+            divisor = divisor * f + left_by[n][DT * 16 + 2][lane_id()] * f2;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * f + left_by[n][dt * 16 + i][lane_id()] * f2;
         }
     }
     sum = both_halves_sum(sum);
@@ -251,6 +285,10 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     const int64_t all_waves = n_seqs * heads * ((n_tokens + 31) / 32);
     const bool room = dtype != MVX_F32 || all_waves <= (dim <= 32 ? 1536 : 768);
     const int waves = dim <= 64 && static_cast<int64_t>(s.left) + s.right < 128 && room ? 1 : 4;
+    // Float32, where a tile's chain of products is three times as long: two waves share the queries of one where that still leaves
+    // every SIMD one wave at most (257 tokens x 4 heads x 64, 33 keys, some hidden: 15.3 -> 12.7 us; 512 x 8 x 64, 127 keys: 18.7 ->
+    // 14.0; 752 waves of 2 x 1500 x 8 x 32, 101 keys: 14.7 -> 21).
+    const bool split = dtype == MVX_F32 && waves == 1 && all_waves <= 512;
     const int q_blocks = static_cast<int>((n_tokens + 32 * waves - 1) / (32 * waves));
     MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
                 name);
@@ -258,17 +296,24 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
         const auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves * (split ? 2 : 1)), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
                                static_cast<T*>(out), lse, reinterpret_cast<T*>(lse != nullptr ? lse + padded_rows(n_seqs * heads * n_tokens) : nullptr));
         };
+        if constexpr (sizeof(T) == 4) {
+            if (split) {
+                dim <= 32 ? launch(window_attention<T, 32, 1, 2>) : launch(window_attention<T, 64, 1, 2>);
+                MVX_CHECK_LAUNCH(name);
+                return MVX_OK;
+            }
+        }
         if (dim <= 32)
-            waves == 1 ? launch(window_attention<T, 32, 1>) : launch(window_attention<T, 32, 4>);
+            waves == 1 ? launch(window_attention<T, 32, 1, 1>) : launch(window_attention<T, 32, 4, 1>);
         else if (dim <= 64)
-            waves == 1 ? launch(window_attention<T, 64, 1>) : launch(window_attention<T, 64, 4>);
+            waves == 1 ? launch(window_attention<T, 64, 1, 1>) : launch(window_attention<T, 64, 4, 1>);
         else if (dim <= 96)
-            launch(window_attention<T, 96, 4>);
+            launch(window_attention<T, 96, 4, 1>);
         else
-            launch(window_attention<T, 128, 4>);
+            launch(window_attention<T, 128, 4, 1>);
         MVX_CHECK_LAUNCH(name);
         return MVX_OK;
     });

@@ -825,3 +825,26 @@ def test_gradients_of_sinks_of_very_many_sequences():
 ], ids=str)
 def test_window_attention_gradients_by_pairs_of_waves(dtype, case):
     test_window_attention(dtype, case)
+
+
+@pytest.mark.parametrize("case", [
+    (1, 33, 1, 1, 64, (0, 0), 0, None, False),       # one tile: the second wave has none
+    (2, 200, 4, 2, 40, (60, 60), 40, (200, 7), True),
+    (1, 640, 8, 1, 32, (100, 20), 100, None, True),  # more tiles of sinks than of the window
+    (3, 5000, 1, 1, 32, (31, 0), 1, None, False),    # 471 waves
+    (3, 5700, 1, 1, 32, (31, 0), 1, None, False),    # 537: single waves again
+], ids=str)
+def test_window_attention_of_queries_shared_by_two_waves(case):
+    test_window_attention(torch.float32, case)
+
+
+def test_queries_shared_by_two_waves_pass_on_what_is_not_finite():
+    q, k, v = (normal(gen(65), (1, 120, 1, 32), torch.float32) for _ in range(3))
+    want, bound = orc.attention(f64(q), f64(k), f64(v), (40, 40), 0, torch.float32)
+    v[0, 3, 0, 5] = float("inf")  # in the first wave's tiles and, 32 keys on, the second's
+    v[0, 40, 0, 6] = float("nan")
+    out = temporal.window_attention(q, k, v, (40, 40))
+    assert (out[0, :44, 0, 5] == float("inf")).all() and out[0, :81, 0, 6].isnan().all()
+    out = f64(out)
+    out[0, :44, 0, 5], out[0, :81, 0, 6] = want[0, :44, 0, 5], want[0, :81, 0, 6]
+    within(out, want, bound, "the other columns and queries")
