@@ -446,7 +446,8 @@ extern "C" int mvx_layer_norm(const void* x, const void* weight, const void* bia
         const int w = static_cast<int>(width);
 #define MVX_NORM(ROW_T, BLOCK, NV)                                                                                             \
     if (p.row_t == ROW_T && p.nv == NV)                                                                                        \
-        hipLaunchKernelGGL((layer_norm_rows<T, ROW_T, BLOCK, NV>), dim3(forward_groups(rows, BLOCK, ROW_T)), dim3(BLOCK), 0, st, xt, weight, bias, param_f32, rows, w, eps, yt, stats)
+        hipLaunchKernelGGL((layer_norm_rows<T, ROW_T, BLOCK, NV>), dim3(forward_groups(rows, BLOCK, ROW_T)), dim3(BLOCK), 0,     \
+                           st, xt, weight, bias, param_f32, rows, w, eps, yt, stats)
         MVX_NORM(64, 256, 1);
         MVX_NORM(64, 256, 2);
         MVX_NORM(64, 256, 4);

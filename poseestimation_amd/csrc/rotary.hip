@@ -9,8 +9,9 @@
 //
 // Bound by memory: q and k are read once and written once in one launch (8 x 4608 tokens x 20 heads of 128 bfloat16: 68 us,
 // 5.5 TB/s; a large copy runs at 5.0).  A workgroup takes a few tokens, computes their cos / sin once into LDS and applies them to
-// all heads of q and k, 16 bytes per access.  Vectors are placed at element alignment with the last one of a stretch moved back to its end (its first values are then written twice, with the same
-// result), so any number of pairs runs at the vector rate; stretches shorter than a vector go element by element.
+// all heads of q and k, 16 bytes per access.  Vectors are placed at element alignment with the last one of a stretch moved back
+// to its end (its first values are then written twice, with the same result), so any number of pairs runs at the vector rate;
+// stretches shorter than a vector go element by element.
 #include <math.h>
 
 #include "element.h"

@@ -34,7 +34,8 @@ constexpr float kSlack = 8.0f;  // in powers of 2; float16 holds weights up to 2
 // kSplit-th tile, kept to itself.
 template <typename T, int DP, int kWaves, int kSplit>
 __global__ __launch_bounds__(64 * kWaves * kSplit, kWaves > 1 && sizeof(T) * DP <= 256 ? 2 : 1) void window_attention(
-    TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest) {
+    TokenTensor q, TokenTensor k, TokenTensor v, AttentionShape a, int q_blocks, T* __restrict__ out, float* __restrict__ lse,
+    T* __restrict__ rest) {
     using Tl = Tiles<T, DP>;
     constexpr int DT = DP / 32, kBQ = 32 * kWaves, kBK = kWaves == 1 ? 32 : kTileRows<T>;  // queries of the workgroup, keys of a tile
     // Copies of the loop over blocks of 32 keys: of longer heads two need more registers than two waves per SIMD have (4 x 4096 x
@@ -295,9 +296,10 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     const unsigned blocks = static_cast<unsigned>(n_seqs * heads * q_blocks);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);
+        T* rest = reinterpret_cast<T*>(lse != nullptr ? lse + padded_rows(n_seqs * heads * n_tokens) : nullptr);
         const auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves * (split ? 2 : 1)), 0, static_cast<hipStream_t>(stream), qt, kt, vt, s, q_blocks,
-                               static_cast<T*>(out), lse, reinterpret_cast<T*>(lse != nullptr ? lse + padded_rows(n_seqs * heads * n_tokens) : nullptr));
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves * (split ? 2 : 1)), 0, static_cast<hipStream_t>(stream), qt, kt,
+                               vt, s, q_blocks, static_cast<T*>(out), lse, rest);
         };
         if constexpr (sizeof(T) == 4) {
             if (split) {

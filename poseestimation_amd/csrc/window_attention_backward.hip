@@ -20,8 +20,8 @@
 //
 // bfloat16, 4 x 4096 x 8 x 64 with 256 keys and 4 sinks: dq 47 us, far queries 12, their sums 5, dk and dv 48; what these have to
 // read and write takes 23, 7, 1 and 20 us at a large copy's rate, the rest is the latency of a few tiles per workgroup.  All keys
-// of 2 x 4096 x 8 x 64: 290 us together (590 Tflop/s of the five products that are counted; two more are computed), of
-// 4096 x 16 x 128, causal: 540 us (320): one wave per SIMD for dk and dv, whose sums alone take half of the registers.
+// of 2 x 4096 x 8 x 64: 295 us together (580 Tflop/s of the five products that are counted; two more are computed), of
+// 4096 x 16 x 128, causal: 424 us (405), one wave per SIMD.
 #include "attention_tiles.h"
 
 namespace mvx {
@@ -34,21 +34,22 @@ constexpr int kBlock = 128;  // queries and keys of a workgroup of four waves; w
 constexpr unsigned kAlone = 0x7fe5a10eu;
 __device__ __forceinline__ bool is_alone(float delta) { return __builtin_bit_cast(unsigned, delta) == kAlone; }
 
-// Copies of a tile's loop over its blocks of 32 rows: of longer heads two need more registers than two waves per SIMD have
-// (4 x 4096 x 8 x 64 bfloat16, 255 keys: dq 50 us with one copy, 47 with two; dk and dv 49 and 48).
-template <int DP, int TILE>
-constexpr int kBlocksOf = DP <= 64 ? TILE / 32 : 1;
+// Both kernels run two blocks of 32 rows of a tile of 64 in one piece of code, and the registers are cut for two waves per SIMD up
+// to heads of 64; longer ones gain more from two blocks in flight in one wave than from a second wave (4096 x 16 x 128 bfloat16,
+// causal: dq 337 us with two waves, 283 with one, 246 with one and two blocks; dk and dv 234 and 219; 2 x 2000 x 8 x 96 float16:
+// 75 and 67 us together.  4 x 4096 x 8 x 64 bfloat16, 255 keys, one block: dq 50 instead of 47, dk and dv 49 instead of 48).
+template <typename T, int DP, int kWaves>
+constexpr int kPerSimd = sizeof(T) * DP <= 128 || (kWaves == 4 && DP <= 64) ? 2 : 1;
 
 // The lowest n bits.
 __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 
 template <typename T, int DP, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 : 128) ? 2 : 1) void window_attention_dq(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o,
-                                                                const T* __restrict__ rest, TokenTensor g, AttentionShape a, float scale, int q_blocks,
-                                                                const float* __restrict__ lse, float* __restrict__ delta,
-                                                                T* __restrict__ dq) {
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window_attention_dq(
+    TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor o, const T* __restrict__ rest, TokenTensor g, AttentionShape a,
+    float scale, int q_blocks, const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq) {
     using Tl = Tiles<T, DP>;
-    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kBlocksOf<DP, kTile>;
+    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kTile / 32;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell k_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell v_tile[2][kTile * Tl::LD];
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -67,9 +68,11 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 :
     const T* kb = static_cast<const T*>(k.p) + seq * k.seq + kv_head * k.head;
     const T* vb = static_cast<const T*>(v.p) + seq * v.seq + kv_head * v.head;
     const bool live = mine < length;
+    const T* q_row = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head;
+    const T* g_row = static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head;
     typename Tl::Frag qf, gf;
-    Tl::load_column(qf, static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head, a.dim, live);
-    Tl::load_column(gf, static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head, a.dim, live);
+    Tl::load_column(qf, q_row, a.dim, live);
+    Tl::load_column(gf, g_row, a.dim, live);
     float my_lse = 0.0f;
     const T* o_row = static_cast<const T*>(o.p) + seq * o.seq + static_cast<int64_t>(mine) * o.token + head * o.head;
     float my_delta;
@@ -79,7 +82,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 :
         Tl::load_column(rf, rest + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim, live);
         my_delta = both_halves_sum(Tl::dot(gf, of, rf));
     } else {
-        my_delta = both_halves_sum(half_dot(static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head, o_row, a.dim, live));
+        my_delta = both_halves_sum(half_dot(g_row, o_row, a.dim, live));
     }
     const int64_t at_row = (seq * a.heads + head) * a.n_tokens + mine;
     if (live) my_lse = lse[at_row];
@@ -164,13 +167,11 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) * DP <= (kWaves == 4 ? 256 :
         }
     }
     if (__any(live && !all_finite(acc))) {
-        const T* qr = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(mine) * q.token + head * q.head;
-        const T* gr = static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(mine) * g.token + head * g.head;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
         for_seen_keys(a, seq, lo, hi, [&](int j) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, kb + j * k.token, a.dim), a.scale_log2, -my_lse));
-            add_row<T, DP>(acc, p * (dot_rows(gr, vb + j * v.token, a.dim) - my_delta), kb + j * k.token, a.dim);
+            const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(q_row, kb + j * k.token, a.dim), a.scale_log2, -my_lse));
+            add_row<T, DP>(acc, p * (dot_rows(g_row, vb + j * v.token, a.dim) - my_delta), kb + j * k.token, a.dim);
         });
     }
     if (mine < a.n_tokens) store_columns<T, DP>(acc, scale, dq + ((seq * a.n_tokens + mine) * a.heads + head) * a.dim, a.dim);
@@ -197,10 +198,9 @@ __device__ __forceinline__ int64_t sink_sums(const AttentionShape& a, int64_t se
 template <typename T, int DP>
 constexpr int kSinkWaves = sizeof(T) * DP > 384 ? 2 : 4;  // float32 heads of 128: 49 KB of tiles per wave
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2 : 1) void window_attention_sinks(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
-                                                                   AttentionShape a, int chunk, int chunks,
-                                                                   const float* __restrict__ lse, const float* __restrict__ delta,
-                                                                   float* __restrict__ partial) {
+__global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2 : 1) void window_attention_sinks(
+    TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g, AttentionShape a, int chunk, int chunks,
+    const float* __restrict__ lse, const float* __restrict__ delta, float* __restrict__ partial) {
     using Tl = Tiles<T, DP>;
     constexpr int kOwn = kSinkWaves<T, DP>;
     struct WaveTiles {
@@ -311,13 +311,12 @@ __global__ __launch_bounds__(256) void window_attention_sinks_join(AttentionShap
 
 // Keys [k0, k0 + 32 kWaves) of one key/value head and the queries of the block's window.
 template <typename T, int DP, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? (DP <= (sizeof(T) == 4 ? 64 : 96)) + 1 : (sizeof(T) * DP <= 128) + 1) void window_attention_dkv(TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g,
-                                                                 AttentionShape a, float scale, int k_blocks, int chunks,
-                                                                 const float* __restrict__ lse, const float* __restrict__ delta,
-                                                                 float* __restrict__ partial,
-                                                                 T* __restrict__ dk, T* __restrict__ dv) {
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window_attention_dkv(
+    TokenTensor q, TokenTensor k, TokenTensor v, TokenTensor g, AttentionShape a, float scale, int k_blocks, int chunks,
+    const float* __restrict__ lse, const float* __restrict__ delta, float* __restrict__ partial, T* __restrict__ dk,
+    T* __restrict__ dv) {
     using Tl = Tiles<T, DP>;
-    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kBlocksOf<DP, kTile>;
+    constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kTile / 32;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell q_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell g_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse, delta
@@ -470,8 +469,8 @@ FarPlan far_plan(int64_t rows, int64_t n_tokens, int64_t left, int64_t sinks) { 
 }
 // Waves of a workgroup of the first and the last kernel, each with 32 queries or keys.  Four share their tiles; where that leaves
 // CUs without work, two take their place if the window is short (4 x 2000 x 2 x 32 float32, 127 keys: 128 workgroups of four 41 us,
-// twice as many of two 34 us; 257 tokens x 4 heads x 64, 33 keys: 24 -> 18 us) or the heads are so long that four waves keep few of
-// their registers (2048 x 4 x 128 bfloat16, all keys: 105 -> 74 us).  Long windows of shorter heads gain from the sharing
+// twice as many of two 34 us; 257 tokens x 4 heads x 64, 33 keys: 24 -> 18 us) or the heads longer than 64 (2048 x 4 x 128
+// bfloat16, all keys: 87 -> 84 us for dk and dv, 70 -> 68 for dq).  Long windows of shorter heads gain from the sharing
 // (2048 x 4 x 64 float32, all keys: 147 and 167 us).
 int waves_of_block(int64_t rows, const AttentionShape& s) {  // rows: sequences times heads
     const bool idle = rows * ((s.n_tokens + kBlock - 1) / kBlock) < 256;
