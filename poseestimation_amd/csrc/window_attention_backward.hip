@@ -13,9 +13,9 @@
 // delta is taken from the output together with what its rounding left: a row that one key dominates has dp - delta near zero
 // there, and the output rounded to bfloat16 alone would be off by as much as the difference (three keys of unit spread: dq and dk
 // off by 0.0033 of their size instead of 0.0025, of twice that spread 0.0066 instead of 0.0024).
-// p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.  (ds in two
-// parts of 16 bits each would bring dq and dk from 0.0024 of their size to 0.0018 of the exact ones in bfloat16, where one rounding
-// of those is 0.0017, at 10 to 20 % more time.)
+// p and ds are rounded to the element type for the products they enter; scores, dp, delta and all sums are float32.  In
+// bfloat16 dq and dk are so off by 0.0024 of their size (one rounding of the exact ones: 0.0017); ds in two parts of 16 bits would
+// give 0.0018, at 10 to 20 % more time.
 // A query that sees a single key weighs it with 1 whatever its score: dp - delta is zero there, but rounding would leave noise,
 // which is all there is where every query sees one key.  The first kernel counts the keys a query sees, gives such a query no
 // gradient, and leaves a mark in the place of its delta.
