@@ -401,16 +401,17 @@ int mvx_rotate_positions(const void* q, const int64_t* q_strides, int q_heads, c
 /*
  * Attention with a sliding window and first tokens that stay visible.  Query i of a sequence sees key j iff j <= i + right and
  * (j >= i - left or j < sinks), j < lengths[sequence] and visible[sequence][j]; out_i = softmax over the seen keys of
- * scale q_i . k_j, times v_j.  A query that sees no key, and a query at or behind its sequence's length, gives zeros.  Values
- * of hidden tokens (not visible, or behind the length) never enter a product, whatever they hold.
+ * scale q_i . k_j, times v_j.  A query that sees no key or whose scores are all minus infinity, and a query at or behind its
+ * sequence's length, gives zeros.  Values of hidden tokens (not visible, or behind the length) never enter a product, whatever
+ * they hold.
  * q            [n_seqs][n_tokens][heads][dim] of dtype; k, v [n_seqs][n_tokens][kv_heads][dim] (head h reads key/value head
  *              h / (heads / kv_heads)); strides {sequence, token, head} in elements (HOST arrays of 3), the last axis
  *              contiguous, base and strides multiples of 16 bytes; dim a multiple of 8, at most 128
  * left, right  >= 0; values beyond n_tokens mean no limit
  * lengths      [n_seqs] int64 or NULL (values outside 0 .. n_tokens are clamped);  visible [n_seqs][n_tokens] bytes or NULL
  * out          [n_seqs][n_tokens][heads][dim], contiguous
- * saved        out: what the backward reads (log2 of the softmax denominators and, with 16-bit types, what the rounding of out
- *              left): mvx_window_attention_saved_bytes() bytes, 16-byte aligned; or NULL
+ * saved        out: what the backward reads (log2 of the softmax denominators, infinity for rows of zeros, and, with 16-bit types,
+ *              what the rounding of out left): mvx_window_attention_saved_bytes() bytes, 16-byte aligned; or NULL
  */
 size_t mvx_window_attention_saved_bytes(int dtype, int64_t n_seqs, int64_t n_tokens, int heads, int dim);
 int mvx_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,

@@ -195,11 +195,15 @@ __global__ __launch_bounds__(64 * kWaves * kSplit, kWaves > 1 && sizeof(T) * DP 
         sum = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
-        // every score a NaN: a finite reference keeps the row apart from one that sees nothing
+        bool nan = false;
         for_seen_keys(a, seq, lo, hi, [&](int j) {
-            top = fmaxf(fmaxf(top, -3.0e38f), dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2);
+            const float x = dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2;
+            nan |= x != x;
+            top = fmaxf(top, x);
         });
-        for_seen_keys(a, seq, lo, hi, [&](int j) {
+        // Scores of minus infinity alone leave an empty row, as if no key were seen; NaN among them do not.
+        if (nan && top == -kInf) top = 0.0f;
+        for_seen_keys(a, seq, lo, top == -kInf ? -1 : hi, [&](int j) {
             const float p = __builtin_amdgcn_exp2f(dot_rows(qr, kb + j * k.token, a.dim) * a.scale_log2 - top);
             sum += p;
             add_row<T, DP>(acc, p, vb + j * v.token, a.dim);
@@ -208,8 +212,8 @@ __global__ __launch_bounds__(64 * kWaves * kSplit, kWaves > 1 && sizeof(T) * DP 
     }
     if (mine >= a.n_tokens) return;
     const bool none = top == -kInf;
-    if (lse != nullptr && half == 0)
-        lse[(seq * a.heads + head) * a.n_tokens + mine] = none ? 0.0f : top + __builtin_amdgcn_logf(sum);  // log2
+    if (lse != nullptr && half == 0)  // log2; an empty row's makes its weights zero
+        lse[(seq * a.heads + head) * a.n_tokens + mine] = none ? kInf : top + __builtin_amdgcn_logf(sum);
     const float factor = none ? 0.0f : 1.0f / divisor;
     const int64_t row = ((seq * a.n_tokens + mine) * a.heads + head) * a.dim;
     store_columns<T, DP>(acc, factor, out + row, a.dim, sizeof(T) == 2 && lse != nullptr ? rest + row : nullptr);

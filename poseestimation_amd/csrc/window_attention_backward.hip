@@ -18,7 +18,8 @@
 // give 0.0018, at 10 to 20 % more time.
 // A query that sees a single key weighs it with 1 whatever its score: dp - delta is zero there, but rounding would leave noise,
 // which is all there is where every query sees one key.  The first kernel counts the keys a query sees, gives such a query no
-// gradient, and leaves a mark in the place of its delta.
+// gradient, and leaves a mark in the place of its delta.  A query whose scores are all minus infinity is an empty row like one
+// that sees no key: its lse is plus infinity, so its weights are zero.
 //
 // bfloat16, 4 x 4096 x 8 x 64 with 256 keys and 4 sinks: dq 47 us, far queries 12, their sums 5, dk and dv 48; what these have to
 // read and write takes 23, 7, 1 and 20 us at a large copy's rate, the rest is the latency of a few tiles per workgroup.  All keys
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
     // not where the key or what it gave is infinite or NaN: 0 times that is NaN
     const bool alone = n_seen == 1 && __builtin_isfinite(my_lse) && __builtin_isfinite(my_delta);
     if (mine < a.n_tokens && half == 0) delta[at_row] = alone ? __builtin_bit_cast(float, kAlone) : my_delta;
-    if (alone) my_lse = __builtin_inff();  // weights of zero: no gradient
+    if (alone) my_lse = kInf;  // weights of zero: no gradient
     v16f acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
@@ -171,7 +172,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
     if (__any(live && !all_finite(acc))) {
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
-        for_seen_keys(a, seq, lo, hi, [&](int j) {
+        // not of an empty row, or one without a gradient: its weights are zero, and zero times an infinite key is a NaN
+        for_seen_keys(a, seq, lo, my_lse == kInf ? -1 : hi, [&](int j) {
             const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(q_row, kb + j * k.token, a.dim), a.scale_log2, -my_lse));
             add_row<T, DP>(acc, p * (dot_rows(g_row, vb + j * v.token, a.dim) - my_delta), kb + j * k.token, a.dim);
         });
@@ -438,6 +440,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
                 const T* qr = static_cast<const T*>(q.p) + seq * q.seq + static_cast<int64_t>(i) * q.token + h * q.head;
                 const T* gr = static_cast<const T*>(g.p) + seq * g.seq + static_cast<int64_t>(i) * g.token + h * g.head;
                 const int64_t at = (seq * a.heads + h) * a.n_tokens + i;
+                if (lse[at] == kInf) continue;  // an empty row
                 const float p = __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, kr, a.dim), a.scale_log2, -lse[at]));
                 if (!is_alone(delta[at])) add_row<T, DP>(dk_acc, p * (dot_rows(gr, vr, a.dim) - delta[at]), qr, a.dim);
                 add_row<T, DP>(dv_acc, p, gr, a.dim);

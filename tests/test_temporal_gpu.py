@@ -848,3 +848,61 @@ def test_queries_shared_by_two_waves_pass_on_what_is_not_finite():
     out = f64(out)
     out[0, :44, 0, 5], out[0, :81, 0, 6] = want[0, :44, 0, 5], want[0, :81, 0, 6]
     within(out, want, bound, "the other columns and queries")
+
+
+def minus_infinity_case(dtype):
+    """Sinks and keys 40 to 59 hold -inf where every query is positive, query 80 holds -inf where every key is: the scores of
+    queries 45 to 59 and 80 are minus infinity alone, those of the others for these keys only."""
+    n, window, sinks = 400, (5, 0), 2
+    g = gen(71)
+    q, k, v, up = (normal(g, (1, n, heads, 32), dtype) for heads in (2, 1, 1, 2))
+    q[..., 3], k[..., 5] = q[..., 3].abs() + 0.5, k[..., 5].abs() + 0.5
+    visible = torch.ones(1, n, dtype=torch.bool)
+    visible[0, :2] = visible[0, 40:60] = False
+    empty = torch.zeros(n, dtype=torch.bool)
+    empty[45:60] = empty[80] = empty[:2] = True
+    plain = [f64(t) for t in (q, k, v, up)]
+    plain[0][:, 80], plain[3][:, 80] = 0, 0
+    want, bound, grads, bounds = orc.attention(*plain[:3], window, sinks, dtype, visible=visible, grad=plain[3])
+    want[:, 80], bound[:, 80] = 0, 0
+    k[0, ~visible[0].to(DEV), :, 3] = -torch.inf
+    q[0, 80, :, 5] = -torch.inf
+    return q, k, v, up, window, sinks, empty, want, bound, grads, bounds
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_of_minus_infinity_alone_give_zeros_and_pass_no_gradient(dtype):
+    q, k, v, up, window, sinks, empty, want, bound, grads, bounds = minus_infinity_case(dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = temporal.window_attention(*leaves, window, sinks)
+    assert (out[0, empty] == 0).all()
+    within(out, want, bound, "out")
+    assert torch.equal(out, temporal.window_attention(*(t.detach() for t in leaves), window, sinks))
+    dq, dk, dv = torch.autograd.grad(out, leaves, up)
+    assert (dq[0, empty] == 0).all()
+    finite = [c for c in range(32) if c != 3]  # zero times the infinite component of the sinks is a NaN
+    within(dq[..., finite], grads[0][..., finite], bounds[0][..., finite], "dq")
+    within(dk, grads[1], bounds[1], "dk")
+    within(dv, grads[2], bounds[2], "dv")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_of_minus_infinity_next_to_a_nan(dtype):
+    q, k, v, up, window, sinks, empty, want, bound, _, _ = minus_infinity_case(dtype)
+    q[0, 50, 0] = float("nan")
+    out = temporal.window_attention(q, k, v, window, sinks)
+    assert out[0, 50, 0].isnan().all() and (out[0, 51:60] == 0).all()
+    out[0, 50, 0] = 0
+    within(out, want, bound, "the others")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_nan_score_is_no_score_of_minus_infinity(dtype):
+    q, k, v = (normal(gen(72), (1, 64, 1, 16), dtype) for _ in range(3))
+    k[0, 10:14, 0, 2] = float("nan")
+    q[0, 30, 0, 0], k[0, 30, 0, 0], k[0, 31, 0, 0] = -torch.inf, 1.0, float("nan")
+    out = temporal.window_attention(q, k, v, (1, 1))
+    nan = [9, 10, 11, 12, 13, 14, 30, 31, 32]
+    assert out[0, nan].isnan().all()
+    rest = [i for i in range(64) if i not in nan]
+    assert torch.isfinite(out[0, rest]).all()
