@@ -203,7 +203,7 @@ __global__ __launch_bounds__(WHOLE ? 64 * kStreamWaves : kThreads) void window_s
         }
         const int64_t head = seq * s.heads + which / parts * group_heads + in_group;
         if (WHOLE) {
-            out[head * s.dim + e] = static_cast<T>(value / sum);
+            out[head * s.dim + e] = static_cast<T>(sum == 0.0f ? 0.0f : value / sum);  // 0: scores of minus infinity alone
         } else {
             shares.values[(head * gridDim.x + blockIdx.x) * s.dim + e] = value;
             if (e == 0) shares.stats[head * gridDim.x + blockIdx.x] = make_float2(top, sum);
@@ -371,9 +371,10 @@ __global__ __launch_bounds__(256) void window_step_join(Shares shares, int n_sha
     __syncthreads();
     if (r == 0) {
         for (int i = 1; i < rows; ++i) value += sums[i * vecs + vec];
-        const float inv = length >= 0 ? 1.0f / total : 0.0f;
+        const bool none = length < 0 || total == 0.0f;  // an idle stream, or scores of minus infinity alone
+        const float inv = none ? 0.0f : 1.0f / total;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[head * dim + vec * 4 + e] = static_cast<T>(length >= 0 ? value[e] * inv : 0.0f);
+        for (int e = 0; e < 4; ++e) out[head * dim + vec * 4 + e] = static_cast<T>(none ? 0.0f : value[e] * inv);
     }
     if (blockIdx.x == 0 && threadIdx.x == 0 && length >= 0) lengths[blockIdx.y] = length + 1;
 }

@@ -906,3 +906,24 @@ def test_a_nan_score_is_no_score_of_minus_infinity(dtype):
     assert out[0, nan].isnan().all()
     rest = [i for i in range(64) if i not in nan]
     assert torch.isfinite(out[0, rest]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,slots", [(64, 40), (32, 1500), (128, 2100)])
+def test_window_attention_step_scores_of_minus_infinity(dtype, dim, slots):
+    g = gen(73)
+    q, k, v = normal(g, (4, 4, dim), dtype).abs() + 0.1, normal(g, (4, 2, dim), dtype), normal(g, (4, 2, dim), dtype)
+    kc, vc = normal(g, (4, slots, 2, dim), dtype), normal(g, (4, slots, 2, dim), dtype)
+    kc[1, :, :, 3] = k[1, :, 3] = -torch.inf  # all keys
+    kc[2, ::2, :, 3] = k[2, :, 3] = -torch.inf  # every other one
+    kc[3, 5, :, 3] = float("nan")
+    lengths = torch.full((4,), 5 * slots + 1, device=DEV)
+    out = temporal.window_attention_step(q, k, v, kc, vc, lengths)
+    assert (out[1] == 0).all() and out[3].isnan().all()
+    for s, kept in ((0, slice(None)), (2, f64(kc)[2, :, 0, 3].isfinite())):
+        keys, values = f64(kc)[s:s + 1, kept], f64(vc)[s:s + 1, kept]
+        n = keys.shape[1]
+        rows = torch.zeros(1, n, 4, dim, dtype=torch.float64)
+        rows[0, -1] = f64(q)[s]
+        want, bound = orc.attention(rows, keys, values, (None, None), 0, dtype)
+        within(out[s], want[0, -1], bound[0, -1], "stream %d" % s)
