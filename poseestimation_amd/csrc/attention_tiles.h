@@ -427,9 +427,11 @@ __device__ __forceinline__ bool sees_all(const AttentionShape& s, int w0, int k0
 
 // ---- pairs one by one -------------------------------------------------------------------------------------------------
 // A product over a tile multiplies what the window hides from a query with a weight of zero, and zero times an infinity or a
-// NaN is a NaN: a value that is not finite would reach queries (or keys) of its tile that do not see it.  Where a wave ends
-// with sums that are not finite it therefore computes its columns again, over the seen pairs alone, with the functions below;
-// the columns that do see such a value then hold what the formula gives, the others their ordinary result.
+// NaN is a NaN: a value that is not finite would reach queries (or keys) of its tile that do not see it.  A column (a query, a
+// key) whose sums end up not finite is therefore computed again, over the pairs it sees alone, with the functions below: if it
+// does see such a value it then holds what the formula gives, otherwise the ordinary result, to rounding.  Columns whose sums
+// are finite met no such value and stay as they are.
+// This walk reads rows lane by lane and is slow.
 
 // Whether the lane's sums are all finite.
 template <int N>
@@ -440,6 +442,11 @@ __device__ __forceinline__ bool all_finite(const v16f (&acc)[N]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) t = fmaf(acc[n][i], 0.0f, t);
     return t == 0.0f;
+}
+// Whether either of the two lanes that share this lane's column says so (called by whole waves).
+__device__ __forceinline__ bool in_either_half(bool v) {
+    const uint64_t b = __ballot(v);
+    return (static_cast<unsigned>(b | b >> 32) >> (lane_id() & 31)) & 1;
 }
 template <typename T>
 __device__ __forceinline__ float dot_rows(const T* a, const T* b, int dim) {

@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * kWaves * kSplit, kWaves > 1 && sizeof(T) * DP 
     }
     sum = both_halves_sum(sum);
     divisor = sizeof(T) == 2 ? both_halves_sum(divisor) : sum;
-    if (__any(mine < length && !(all_finite(acc) && divisor < kInf))) {
+    if (in_either_half(mine < length && !(all_finite(acc) && divisor < kInf))) {
         const T* qr = qb + static_cast<int64_t>(mine) * q.token;
         top = -kInf;
         sum = 0.0f;

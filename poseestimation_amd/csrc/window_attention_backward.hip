@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
             Tl::cols_times(pool, s, acc);
         }
     }
-    if (__any(live && !all_finite(acc))) {
+    if (in_either_half(live && !all_finite(acc))) {
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
         // not of an empty row, or one without a gradient: its weights are zero, and zero times an infinite key is a NaN
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
             Tl::cols_times(pool, dp, dk_acc);
         }
     }
-    if (__any(kept && !(all_finite(dk_acc) && all_finite(dv_acc)))) {
+    if (in_either_half(kept && !(all_finite(dk_acc) && all_finite(dv_acc)))) {
         const T* kr = static_cast<const T*>(k.p) + seq * k.seq + static_cast<int64_t>(mine) * k.token + kv_head * k.head;
         const T* vr = static_cast<const T*>(v.p) + seq * v.seq + static_cast<int64_t>(mine) * v.token + kv_head * v.head;
 #pragma unroll

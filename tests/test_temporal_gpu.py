@@ -927,3 +927,31 @@ def test_window_attention_step_scores_of_minus_infinity(dtype, dim, slots):
         rows[0, -1] = f64(q)[s]
         want, bound = orc.attention(rows, keys, values, (None, None), 0, dtype)
         within(out[s], want[0, -1], bound[0, -1], "stream %d" % s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_beside_one_that_is_not_finite_keep_their_bits(dtype):
+    n, window, sinks = 300, (20, 6), 2
+    g = gen(74)
+    q, k, v, up = (normal(g, (1, n, heads, 64), dtype) for heads in (2, 1, 1, 2))
+
+    def both(q, up):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        out = temporal.window_attention(*leaves, window, sinks)
+        return [out.detach(), *torch.autograd.grad(out, leaves, up)]
+
+    clean = both(q, up)
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[[7, 133, 290]] = True
+    q2, up2 = q.clone(), up.clone()
+    q2[0, 7, 0, 1], q2[0, 133] = float("nan"), float("nan")
+    up2[0, 290, 1, 0] = float("inf")
+    out, dq, dk, dv = both(q2, up2)
+    assert out[0, [7, 133], 0].isnan().all()
+    assert torch.equal(out[0, ~bad], clean[0][0, ~bad]) and torch.equal(dq[0, ~bad], clean[1][0, ~bad])
+    beyond = ~orc.seen_pairs(n, *window, sinks, None, None)[bad].any(0)  # keys that none of the three sees
+    assert beyond.sum() > 200
+    # those of its tiles are computed again: the same to rounding
+    _, _, grads, bounds = orc.attention(f64(q), f64(k), f64(v), window, sinks, dtype, grad=f64(up))
+    for name, a, c, e in zip(("dk", "dv"), (dk, dv), grads[1:], bounds[1:]):
+        within(a[0, beyond], c[0, beyond], e[0, beyond], name)
