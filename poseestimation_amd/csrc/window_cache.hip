@@ -289,11 +289,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_step_tiles(const T* __rest
         }
         const float ref = top == -kInf ? 0.0f : top;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], s.scale_log2, -ref));
-            sum += x[i];
-        }
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], s.scale_log2, -ref));
         Tl::cols_times(pool, x, acc);
+        sum = Tl::rounded_sum(x, sum);  // of the weights as the product takes them: the result stays a mean of the values
     }
     sum = both_halves_sum(sum);
     __syncthreads();  // the tiles are read: their memory takes the sums

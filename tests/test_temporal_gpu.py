@@ -955,3 +955,29 @@ def test_queries_beside_one_that_is_not_finite_keep_their_bits(dtype):
     _, _, grads, bounds = orc.attention(f64(q), f64(k), f64(v), window, sinks, dtype, grad=f64(up))
     for name, a, c, e in zip(("dk", "dv"), (dk, dv), grads[1:], bounds[1:]):
         within(a[0, beyond], c[0, beyond], e[0, beyond], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_window_attention_step_is_a_mean_of_the_values(dtype, dim):
+    """Of every 32 keys 31 have the same score, so their weights are rounded alike; the values are of one size, so a mean of them
+    is off by little more than its own rounding: u |o|, and relative errors u of the weights move it by 2 u sum p |v - o| at most.
+    Scores are off by (dim + 4) 2^-24 sum |q||k| scale, sums over the slots by slots 2^-24."""
+    g = gen(75 + dim)
+    b, heads, slots, scale = 2, 16, 3008, dim ** -0.5
+    q, top, low = normal(g, (b, heads, dim), dtype), normal(g, (dim,), dtype), normal(g, (dim,), dtype)
+    kc = low.expand(b, slots, 1, dim).contiguous()
+    kc[:, ::32] = top
+    u = torch.finfo(dtype).eps / 2
+    vc = (1.5 + 2 * u * torch.randint(0, 3, (b, slots, 1, dim), generator=g)).to(dtype).to(DEV)
+    k, v = kc[:, 0].clone(), vc[:, 0].clone()
+    lengths = torch.full((b,), 5 * slots, device=DEV)  # the new token goes to slot 0 and is what lies there
+    out = f64(temporal.window_attention_step(q, k, v, kc, vc, lengths))
+    for s in range(b):
+        keys, values, rows = f64(kc)[s, :, 0], f64(vc)[s, :, 0], f64(q)[s]
+        p = torch.softmax(rows @ keys.T * scale, -1)
+        want = p @ values
+        apart = (p[:, :, None] * (values[None] - want[:, None]).abs()).sum(1)
+        score = (dim + 4) * 2.0 ** -24 * scale * (rows.abs() @ keys.abs().T).amax()
+        bound = u * want + 2 * u * apart * (1 + u) + want * slots * 2.0 ** -24 + 2 * score * apart
+        within(out[s], want, bound, "stream %d" % s)
