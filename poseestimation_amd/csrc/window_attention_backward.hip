@@ -44,6 +44,45 @@ __device__ __forceinline__ bool is_alone(float delta) { return __builtin_bit_cas
 template <typename T, int DP, int kWaves>
 constexpr int kPerSimd = sizeof(T) * DP <= 128 || (kWaves == 4 && DP <= 64) ? 2 : 1;
 
+// float16 is exact to its half step from 2^-14 to 2^16 only, and score gradients may lie anywhere: as small as the weights of a
+// long window times what the loss left, as large as its scaling made them.  Every column (a query for dq, a key for dk) therefore
+// carries its sums times a power of two: the first block of score gradients above 2^(15 - kFirstPower) brings its largest to
+// 2^5 .. 2^6, which leaves 19 binades below it, and one that passes 2^15 later lowers the power again, with the sums so far.
+// Weights are at most 1 and enter dv times 2^kWeightPower.  The other types have float32's range and no power.
+// Without it (4096 causal tokens, gradients of 1e-3 and 1e-4) dq and dk are off by 0.0016 and 0.016 of their size instead of 0.0004
+// and 0.0028, of which one rounding of the exact ones is 0.0003 and 0.0028, and score gradients beyond 65504 are infinite.  It costs
+// the largest of 16 values and, for dk, a product each: 4 x 4096 x 8 x 64 with 255 keys 113 -> 119 us, all keys of 2 x 4096 x 8 x 64
+// 299 -> 317, 4096 x 16 x 128 causal 423 -> 482.
+template <typename T>
+constexpr bool kScaled = std::is_same_v<T, f16>;
+template <typename T>
+constexpr int kFirstPower = kScaled<T> ? 60 : 0;
+template <typename T>
+constexpr int kWeightPower = kScaled<T> ? 14 : 0;
+
+// Lowers the powers where the block `ds`, already times 2^power, needs it; whether any lane's has moved.
+template <int N>
+__device__ __forceinline__ bool fit(v16f& ds, int& power, v16f (&acc)[N]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(most, fabsf(ds[i])), fabsf(ds[i + 1]));
+    if (__builtin_expect(!__any(most > 0x1p15f), 1)) return false;
+    most = both_halves_max(most);
+    const int by = most > 0x1p15f && most < kInf ? 6 - __builtin_amdgcn_frexp_expf(most) : 0;
+    const float f = __builtin_amdgcn_ldexpf(1.0f, by);
+    power += by;
+    ds *= f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] *= f;
+    return true;
+}
+template <int N>
+__device__ __forceinline__ void unscale(v16f (&acc)[N], int power) {
+    const float f = __builtin_amdgcn_ldexpf(1.0f, -power);
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] *= f;
+}
+
 // The lowest n bits.
 __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 
@@ -109,6 +148,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
     v16f acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
+    int power = kFirstPower<T>;
+    float shift = kScaled<T> ? static_cast<float>(power) - my_lse : -my_lse;
 
     TileInFlight<T, DP, kTile, kThreads> k_next, v_next;
     k_next.place(k.token, a.dim);
@@ -158,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
             Tl::cols(pool, kt + 32 * b * Tl::LD);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -my_lse)) * (dp[i] - my_delta);
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, shift)) * (dp[i] - my_delta);
             if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -166,9 +207,12 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
                     s[i] = (r <= hi_r) & ((r >= lo_r) | (r < sink_r)) & ((bits >> r) & 1) ? s[i] : 0.0f;
                 }
             }
+            if constexpr (kScaled<T>)
+                if (fit(s, power, acc)) shift = static_cast<float>(power) - my_lse;
             Tl::cols_times(pool, s, acc);
         }
     }
+    if constexpr (kScaled<T>) unscale(acc, power);
     if (in_either_half(live && !all_finite(acc))) {
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = v16f{};
@@ -237,6 +281,8 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2
     v16f dk_acc[DP / 32], dv_acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+    int power = kFirstPower<T> - kWeightPower<T>;
+    float gain = __builtin_amdgcn_ldexpf(1.0f, power);
 
     WaveTiles& tile = shared.wave[wave];
     TileInFlight<T, DP, 32, 64> q_next, g_next;
@@ -251,7 +297,7 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's reads of the last tile come before these writes
         q_next.store(tile.q);
         g_next.store(tile.g);
-        tile.stats[half][lane & 31] = stat;
+        tile.stats[half][lane & 31] = half == 0 ? stat - kWeightPower<T> : stat;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         typename Tl::Pool pool;
         Tl::rows(pool, tile.q);
@@ -267,7 +313,8 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * i4 + e;
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e])), ds = p * (dp[i] - d4[e]);
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e]));
+                const float ds = (kScaled<T> ? p * gain : p) * (dp[i] - d4[e]);
                 const bool seen = kept && 8 * i4 + e < rows;
                 s[i] = seen ? p : 0.0f;
                 dp[i] = seen && !is_alone(d4[e]) ? ds : 0.0f;
@@ -275,7 +322,13 @@ __global__ __launch_bounds__(64 * (kSinkWaves<T, DP>), sizeof(T) * DP <= 192 ? 2
         }
         Tl::cols_times(pool, s, dv_acc);
         Tl::cols(pool, tile.q);
+        if constexpr (kScaled<T>)
+            if (fit(dp, power, dk_acc)) gain = __builtin_amdgcn_ldexpf(1.0f, power);
         Tl::cols_times(pool, dp, dk_acc);
+    }
+    if constexpr (kScaled<T>) {
+        unscale(dk_acc, power + kWeightPower<T>);
+        unscale(dv_acc, kWeightPower<T>);
     }
     __syncthreads();
     for (int w = 0; w < kOwn; ++w) {
@@ -323,7 +376,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
     constexpr int kThreads = 64 * kWaves, kMine = 32 * kWaves, kTile = kTileRows<T>, kBlocks = kTile / 32;
     __shared__ __attribute__((aligned(16))) typename Tl::Cell q_tile[2][kTile * Tl::LD];
     __shared__ __attribute__((aligned(16))) typename Tl::Cell g_tile[2][kTile * Tl::LD];
-    __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse, delta
+    __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // of a tile: lse - kWeightPower, delta
     unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int block = id % k_blocks;
     id /= k_blocks;
@@ -348,7 +401,10 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
     const int wave_last = w0 < a.sinks ? length - 1 : min(w0 + 31 + a.left, length - 1);
 
     v16f dk_acc[DP / 32], dv_acc[DP / 32];
-    if (w0 < a.sinks && end < length) {  // what the queries behind the window give the sinks
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
+    const auto add_far_queries = [&] {  // what the queries behind the window give the sinks
+        if (w0 >= a.sinks || end >= length) return;
         float* sums = partial + sink_sums<DP>(a, seq, kv_head, w0 / 32, chunks);
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
@@ -356,12 +412,12 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
             for (int i4 = 0; i4 < 4; ++i4) {
                 const v4f k4 = *sink_vec<DP>(sums, dt, i4, 0), v4 = *sink_vec<DP>(sums, dt, i4, 1);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) dk_acc[dt][4 * i4 + e] = k4[e], dv_acc[dt][4 * i4 + e] = v4[e];
+                for (int e = 0; e < 4; ++e) dk_acc[dt][4 * i4 + e] += k4[e], dv_acc[dt][4 * i4 + e] += v4[e];
             }
-    } else {
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) dk_acc[dt] = dv_acc[dt] = v16f{};
-    }
+    };
+    if constexpr (!kScaled<T>) add_far_queries();
+    int power = kFirstPower<T> - kWeightPower<T>;
+    float gain = __builtin_amdgcn_ldexpf(1.0f, power);
 
     TileInFlight<T, DP, kTile, kThreads> q_next, g_next;
     q_next.place(q.token, a.dim);
@@ -374,6 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
         const int r = i0 + (threadIdx.x & (kTile - 1));
         if (threadIdx.x < 2 * kTile)
             stat_next = r < end ? (threadIdx.x < kTile ? lse : delta)[(seq * a.heads + head) * a.n_tokens + r] : 0.0f;
+        if (kScaled<T> && threadIdx.x < kTile) stat_next -= kWeightPower<T>;
     };
     const auto put = [&](int t) {
         q_next.store(q_tile[t & 1]);
@@ -412,7 +469,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
                 for (int e = 0; e < 4; ++e) {
                     const int i = 4 * i4 + e;
                     s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -l4[e]));
-                    dp[i] = s[i] * (dp[i] - d4[e]);
+                    dp[i] = (kScaled<T> ? s[i] * gain : s[i]) * (dp[i] - d4[e]);
                 }
             }
             if (!whole) {
@@ -427,8 +484,15 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
             }
             Tl::cols_times(pool, s, dv_acc);
             Tl::cols(pool, qt + 32 * b * Tl::LD);
+            if constexpr (kScaled<T>)
+                if (fit(dp, power, dk_acc)) gain = __builtin_amdgcn_ldexpf(1.0f, power);
             Tl::cols_times(pool, dp, dk_acc);
         }
+    }
+    if constexpr (kScaled<T>) {
+        unscale(dk_acc, power + kWeightPower<T>);
+        unscale(dv_acc, kWeightPower<T>);
+        add_far_queries();
     }
     if (in_either_half(kept && !(all_finite(dk_acc) && all_finite(dv_acc)))) {
         const T* kr = static_cast<const T*>(k.p) + seq * k.seq + static_cast<int64_t>(mine) * k.token + kv_head * k.head;

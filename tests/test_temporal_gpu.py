@@ -981,3 +981,43 @@ def test_window_attention_step_is_a_mean_of_the_values(dtype, dim):
         score = (dim + 4) * 2.0 ** -24 * scale * (rows.abs() @ keys.abs().T).amax()
         bound = u * want + 2 * u * apart * (1 + u) + want * slots * 2.0 ** -24 + 2 * score * apart
         within(out[s], want, bound, "stream %d" % s)
+
+
+@pytest.mark.parametrize("size", [3e4, 1.0, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("n,dim,window,sinks,heads,kv_heads", [(4000, 64, (None, 0), 0, 1, 1), (1500, 128, (None, None), 0, 1, 1),
+                                                               (2500, 32, (900, 0), 3, 2, 1), (1200, 96, (1, 1), 0, 1, 1)])
+def test_float16_gradients_of_any_size(n, dim, window, sinks, heads, kv_heads, size):
+    """What the type's range does to the score gradients must not be seen in the results: each is off by half a step relative to
+    itself (u), or by 2^-30 of the largest in its row (dq) or column (dk); weights likewise by u or 2^-39.  With the forward's
+    weights off by u, delta = g . o is off by u sum |g| sum p |v - o|, and by u^2 |g| |o| and 2^-25 |g| of what two roundings leave
+    of o.  float32: scores (dim + 4) 2^-24 sum |q||k| scale, sums 2^-24 per term.  A result is rounded to u or 2^-25."""
+    dtype = torch.float16
+    g = gen(n + dim)
+    q, k, v = (normal(g, (1, n, h, dim), dtype, True) for h in (heads, kv_heads, kv_heads))
+    up = (torch.randn((1, n, heads, dim), generator=g) * size).clamp(-6e4, 6e4).to(dtype).to(DEV)
+    got = [f64(t)[0] for t in torch.autograd.grad(temporal.window_attention(q, k, v, window, sinks), (q, k, v), up)]
+    u, e, scale = 2.0 ** -11, 2.0 ** -24, dim ** -0.5
+    seen = orc.seen_pairs(n, *window, sinks, None, None)
+    want = [torch.zeros_like(t) for t in got]
+    bound = [torch.zeros_like(t) for t in got]
+    for h in range(heads):
+        at = h * kv_heads // heads
+        qh, kh, vh, gh = f64(q)[0, :, h], f64(k)[0, :, at], f64(v)[0, :, at], f64(up)[0, :, h]
+        p = torch.softmax((qh @ kh.T * scale).masked_fill(~seen, -torch.inf), -1)
+        o, dp = p @ vh, gh @ vh.T
+        ds = p * (dp - (gh * o).sum(-1, keepdim=True))
+        x = 2 * (dim + 4) * e * scale * torch.where(seen, qh.abs() @ kh.abs().T, 0.0).amax(-1, keepdim=True) + 64 * e + n * e
+        spread = (p @ vh ** 2 - o ** 2).clamp(min=0).sqrt()  # at least sum p |v - o|
+        delta = (gh.abs() * (u * spread * (1 + 4 * u) + (u * u + 2 * x) * o.abs() + 2.0 ** -25)).sum(-1, keepdim=True)
+        off = (u + x) * ds.abs() + p * (1 + u) * (delta + (dim + 4) * e * torch.where(seen, gh.abs() @ vh.abs().T, 0.0))
+        rows, cols = (2.0 ** -30 * seen * (ds.abs() + off).amax(d, keepdim=True) for d in (1, 0))
+        want[0][:, h] = scale * ds @ kh
+        bound[0][:, h] = scale * (off + rows + n * e * ds.abs()) @ kh.abs()
+        want[1][:, at] += scale * ds.T @ qh
+        bound[1][:, at] += scale * (off + cols + n * heads * e * ds.abs()).T @ qh.abs()
+        want[2][:, at] += p.T @ gh
+        bound[2][:, at] += ((u + x + n * heads * e) * p + 2.0 ** -39 * seen).T @ gh.abs()
+    for name, a, c, b in zip(("dq", "dk", "dv"), got, want, bound):
+        over = (c.abs() + b) * (1 + u) > 65504  # beyond the type
+        within(torch.where(over, 0.0, a), torch.where(over, 0.0, c), b + u * (c.abs() + b) + 2.0 ** -25, name)
+        assert over.double().mean() < 0.5
