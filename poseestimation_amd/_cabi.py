@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmvx.so")
@@ -143,6 +144,13 @@ def forward_only(what, *tensors):
     if needs_grad(*tensors):
         raise MvxError("%s is forward-only (no backward kernel): call it under torch.no_grad() or detach its inputs; "
                        "training through this operation needs the reference's differentiable torch ops" % what)
+
+
+def no_tangents(what, *tensors):
+    """Raises when one of `tensors` carries a forward-mode tangent (its requires_grad is False): the kernels have no
+    forward-mode derivative, and a result without a tangent would stand for a derivative of zero."""
+    if forward_ad._current_level >= 0 and any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise MvxError("%s has no forward-mode derivative: an input carries a tangent" % what)
 
 
 def ptr(t):

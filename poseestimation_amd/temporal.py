@@ -11,7 +11,7 @@ of the voxel grid -- needs around its matrix products.  The reference has no suc
 Tensors are float32, bfloat16 or float16 HIP tensors, tokens are (batch, tokens, heads, head_dim).  Arithmetic, sums and
 softmax statistics are float32, results are rounded once to the input's type.  Calls are asynchronous on torch's current
 stream of the tensors' device and can be captured into a graph.  layer_norm, rotate_positions and window_attention are
-differentiable (once) by backward kernels whose sums run in a fixed order.
+differentiable (once) by backward kernels whose sums run in a fixed order; inputs with forward-mode tangents are refused.
 """
 import ctypes
 import functools
@@ -181,6 +181,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         _norm_check(x, weight, bias, eps)
         param = weight if weight is not None else bias
         param_f32 = int(param is not None and param.dtype == torch.float32)
+    _cabi.no_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and _cabi.needs_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps), param_f32)
     return _norm_run(x, weight, bias, eps, param_f32, False)[1]
@@ -281,6 +282,7 @@ def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum
     sections = tuple(map(int, sections))
     if not _rotate_usual(q, k, positions, sections, base):
         _rotate_check(q, k, positions, sections, base)
+    _cabi.no_tangents("rotate_positions", q, k, positions)
     positions = positions.contiguous()
     how = (sections, float(base), int(bool(shared_spectrum)), int(bool(pairs)))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
@@ -416,6 +418,7 @@ def window_attention(q, k, v, window, sinks=0, *, lengths=None, visible=None, sc
             _cabi.same_device(q, "q", visible=visible)
         visible = visible.contiguous()
     how = (min(int(left), n), min(int(right), n), min(_check_sinks(sinks), n), _check_scale(scale, dim))
+    _cabi.no_tangents("window_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, lengths, visible, how)
     return _window_run(q, k, v, lengths, visible, how, False)[3]
@@ -474,6 +477,7 @@ def window_cache_fill(k, v, k_cache, v_cache, lengths, sinks=0):
     _check_lengths(lengths, b, k, "k")
     if torch.is_grad_enabled():
         _cabi.forward_only("window_cache_fill", k, v, k_cache, v_cache)
+    _cabi.no_tangents("window_cache_fill", k, v, k_cache, v_cache)
     k, v, lengths = _tokens(k), _tokens(v), lengths.contiguous()
     _run(k.get_device(), "window_cache_fill", "mvx_window_cache_fill", k.data_ptr(), _strides(k), v.data_ptr(), _strides(v),
          _DTYPES[k.dtype], lengths.data_ptr(), b, n, kv_heads, dim, k_cache.shape[1] - sinks, sinks, k_cache.data_ptr(),
@@ -508,6 +512,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks=0, *, scale=
         raise ValueError("lengths must be contiguous: it is written in place")
     if torch.is_grad_enabled():
         _cabi.forward_only("window_attention_step", q, k, v, k_cache, v_cache)
+    _cabi.no_tangents("window_attention_step", q, k, v, k_cache, v_cache)
     scale = _check_scale(scale, dim)
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     if q.data_ptr() % 16:

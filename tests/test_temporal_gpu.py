@@ -4,6 +4,7 @@ import itertools
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import temporal_oracle as orc
 from poseestimation_amd import _cabi, temporal
@@ -1021,3 +1022,26 @@ def test_float16_gradients_of_any_size(n, dim, window, sinks, heads, kv_heads, s
         over = (c.abs() + b) * (1 + u) > 65504  # beyond the type
         within(torch.where(over, 0.0, a), torch.where(over, 0.0, c), b + u * (c.abs() + b) + 2.0 ** -25, name)
         assert over.double().mean() < 0.5
+
+
+def test_forward_mode_tangents_are_refused():
+    """No operator has a forward-mode rule: a result without a tangent would be a derivative of zero."""
+    x, w, t = torch.randn(1, 6, 2, 16, device=DEV), torch.randn(16, device=DEV), torch.randn(1, 6, 2, 16, device=DEV)
+    positions, lengths = torch.zeros(6, 1, device=DEV), torch.ones(1, dtype=torch.int64, device=DEV)
+    kc, vc = torch.zeros(1, 9, 2, 16, device=DEV), torch.zeros(1, 9, 2, 16, device=DEV)
+    plain = temporal.window_attention(x, x, x, (2, 0))
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), fwd.dual_level():
+            d, dw = fwd.make_dual(x, t), fwd.make_dual(w, w)
+            for call in (lambda: temporal.layer_norm(d), lambda: temporal.layer_norm(x, dw), lambda: temporal.layer_norm(x, w, dw),
+                         lambda: temporal.rotate_positions(d, None, positions, (8,)), lambda: temporal.rotate_positions(x, d, positions, (8,)),
+                         lambda: temporal.rotate_positions(x, x, fwd.make_dual(positions, positions), (8,)),
+                         lambda: temporal.window_attention(d, x, x, (2, 0)), lambda: temporal.window_attention(x, d, x, (2, 0)),
+                         lambda: temporal.window_attention(x, x, d, (2, 0)),
+                         lambda: temporal.window_cache_fill(d, x, kc, vc, lengths), lambda: temporal.window_cache_fill(x, d, kc, vc, lengths),
+                         lambda: temporal.window_attention_step(d[:, 0], x[:, 0], x[:, 0], kc, vc, lengths),
+                         lambda: temporal.window_attention_step(x[:, 0], x[:, 0], d[:, 0], kc, vc, lengths)):
+                with pytest.raises(_cabi.MvxError, match="tangent"):
+                    call()
+            assert torch.equal(temporal.window_attention(x, x, x, (2, 0)), plain)  # no tangent: as ever
+    assert (kc == 0).all() and lengths.item() == 1
