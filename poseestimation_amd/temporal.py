@@ -279,7 +279,10 @@ def rotate_positions(q, k, positions, sections, *, base=10000.0, shared_spectrum
     i turns by position[axis] * base ** -e, with e its place in the axis' section over the section's pairs or, with
     shared_spectrum, i over all pairs.  Pairs are (i, i + all pairs), or neighbours (2i, 2i + 1) with pairs=True.  Angles are
     float64, so positions of millions keep their place.  Differentiable with respect to q and k."""
-    sections = tuple(map(int, sections))
+    given = tuple(sections)
+    sections = tuple(map(int, given))
+    if given != sections:
+        raise ValueError("sections must be whole numbers of pairs, got %r" % (given,))
     if not _rotate_usual(q, k, positions, sections, base):
         _rotate_check(q, k, positions, sections, base)
     _cabi.no_tangents("rotate_positions", q, k, positions)

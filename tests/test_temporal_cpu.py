@@ -153,3 +153,13 @@ def test_a_ring_whose_size_passes_64_bits_is_refused():
     for window, sinks in ((big, 1), (1, big), (big, big)):
         assert lib.mvx_window_attention_step(SOME, SOME, SOME, 0, 1, 1, 1, 8, window, sinks, 1.0, SOME, SOME, SOME, SOME, None, 0,
                                              None) == UNSUPPORTED
+
+
+def test_sections_of_parts_of_pairs_are_refused():
+    t, positions = torch.zeros(1, 4, 2, 16), torch.zeros(4, 2)
+    for sections in ((4.5, 3), (3.999, 4), ("4", "4"), (4, True + 0.5)):
+        with pytest.raises(ValueError, match="whole numbers"):
+            temporal.rotate_positions(t, None, positions, sections)
+    for sections in ((4, 4), (4.0, 4.0), [4, 4], torch.tensor([4, 4])):
+        with pytest.raises(_cabi.MvxError, match="HIP device only"):  # taken; what is refused is the CPU tensor
+            temporal.rotate_positions(t, None, positions, sections)
