@@ -387,7 +387,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
     const int length = seq_length(a, seq);
     const int k0 = block * kMine, w0 = k0 + wave * 32, mine = w0 + (lane_id() & 31);
     const int begin = max(0, k0 - a.right);
-    const int end = k0 < a.sinks ? window_end(a, k0 / kBlock * kBlock, length) : min(length, k0 + kMine + a.left);
+    // without chunks the sinks' block walks their far queries itself
+    const int end = k0 >= a.sinks ? min(length, k0 + kMine + a.left) : chunks > 0 ? window_end(a, k0 / kBlock * kBlock, length) : length;
     const int per_head = begin < end && k0 < length ? (end - begin + kTile - 1) / kTile : 0, tiles = per_head * share;
 
     const bool kept = mine < length && (a.visible == nullptr || a.visible[seq * a.n_tokens + mine] != 0);
@@ -519,7 +520,12 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, DP, kWaves>)) void window
 
 // How the queries behind the windows of the sinks are cut: chunks of 128, one round of a workgroup's waves, where all of them
 // run at once (two workgroups per CU), else of 256 (4 x 4096 x 8 x 64 bfloat16: 11.7 against 16.5 us; 4 x 2000 x 2 x 32 float32:
-// 14.4 against 9.6 us with chunks of 128); at most 32 chunks.
+// 14.4 against 9.6 us with chunks of 128); at most 32 chunks.  A chunk of 32 sinks leaves 8 KB (heads of 32) to 32 KB (of 128):
+// together no more than what 2048 of them take or a quarter of the gradients of 16-bit keys and values, whichever is more, but one
+// chunk in any case (8192 tokens x 8 x 64 bfloat16, 127 keys, 1000 sinks: backward 211 -> 142 us for it).
+// Where many sinks fill the GPU with their blocks alone there are no chunks, and the kernel of the keys walks all queries (8192 x 8
+// x 128 bfloat16, all of them sinks: 1227 us with two chunks, 724 with none; few sinks leave three of its four waves without work,
+// 128 x 2048 x 8 x 64 with four of them: 1150 and 1593).
 struct FarPlan {
     int sink_blocks, chunk, chunks;
 };
@@ -530,8 +536,13 @@ FarPlan far_plan(int64_t rows, int64_t n_tokens, int64_t left, int64_t sinks) { 
     const int64_t far = n_tokens - kBlock - left;
     if (sinks <= 0 || far <= 0) return f;
     f.sink_blocks = static_cast<int>((sinks + 31) / 32);
-    int64_t chunk = rows * f.sink_blocks * ((far + 127) / 128) <= 512 ? 128 : 256;
-    if (chunk * 32 < far) chunk = ((far + 31) / 32 + 127) / 128 * 128;
+    const int64_t blocks = rows * f.sink_blocks;
+    if (f.sink_blocks >= kBlock / 32 && blocks > 1024) return f;
+    int64_t most = 2048 / blocks, share = n_tokens / (256 * f.sink_blocks);
+    if (most < share) most = share;
+    most = most < 1 ? 1 : (most > 32 ? 32 : most);
+    int64_t chunk = blocks * ((far + 127) / 128) <= 512 ? 128 : 256;
+    if (chunk * most < far) chunk = ((far + most - 1) / most + 127) / 128 * 128;
     f.chunk = static_cast<int>(chunk);
     f.chunks = static_cast<int>((far + chunk - 1) / chunk);
     return f;

@@ -163,3 +163,17 @@ def test_sections_of_parts_of_pairs_are_refused():
     for sections in ((4, 4), (4.0, 4.0), [4, 4], torch.tensor([4, 4])):
         with pytest.raises(_cabi.MvxError, match="HIP device only"):  # taken; what is refused is the CPU tensor
             temporal.rotate_positions(t, None, positions, sections)
+
+
+def test_backward_workspace_stays_small_with_many_sinks():
+    """The sums of the sinks' far queries (256 bytes per chunk of 32 sinks and value of a head): at most those of 2048 chunks, or a
+    byte per token and value, or one chunk for each of up to three blocks of sinks."""
+    size = _cabi.load().mvx_window_attention_backward_workspace_bytes
+    for seqs in (1, 6, 300):
+        for n in (300, 8192, 100000):
+            for kv_heads, dim in ((1, 128), (8, 128), (16, 64), (4, 40)):
+                for left in (0, 255, n // 2):
+                    for sinks in (0, 1, 33, 130, 1000, n):
+                        rows, wide = seqs * kv_heads, (dim + 31) // 32 * 32
+                        sums = size(seqs, n, kv_heads, kv_heads, dim, left, sinks) - 4 * ((rows * n + 3) // 4 * 4)
+                        assert 0 <= sums <= wide * max(2048 * 256, rows * n, rows * 256 * min(3, (sinks + 31) // 32)), (seqs, n, kv_heads, dim, left, sinks)

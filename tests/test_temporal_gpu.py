@@ -1045,3 +1045,22 @@ def test_forward_mode_tangents_are_refused():
                     call()
             assert torch.equal(temporal.window_attention(x, x, x, (2, 0)), plain)  # no tangent: as ever
     assert (kc == 0).all() and lengths.item() == 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [
+    (12, 1500, 4, 4, 16, (0, 0), 1490, (1500, 900) * 6, False),   # blocks of sinks alone fill the GPU
+    (2, 1100, 8, 4, 32, (40, 3), 1100, (1100, 1024), True),       # every token a sink
+    (1, 2300, 1, 1, 64, (7, 0), 1000, None, False),               # few chunks of many sinks
+], ids=str)
+def test_window_attention_gradients_of_many_sinks(dtype, case):
+    q, k, v, up, lengths, visible = attention_case(case, dtype, leaf=True)
+    out = temporal.window_attention(q, k, v, case[5], case[6], lengths=on_gpu(lengths), visible=on_gpu(visible))
+    got = torch.autograd.grad(out, (q, k, v), up)
+    for s in {0, case[0] - 1}:
+        one = slice(s, s + 1)
+        _, _, grads, bounds = orc.attention(f64(q)[one], f64(k)[one], f64(v)[one], case[5], case[6], dtype,
+                                            None if lengths is None else lengths[one], None if visible is None else visible[one],
+                                            grad=f64(up)[one])
+        for name, a, c, e in zip(("dq", "dk", "dv"), got, grads, bounds):
+            within(a[one], c, e, "%s of sequence %d" % (name, s))
