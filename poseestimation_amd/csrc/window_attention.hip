@@ -295,7 +295,8 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     // 14.0; 752 waves of 2 x 1500 x 8 x 32, 101 keys: 14.7 -> 21).
     const bool split = dtype == MVX_F32 && waves == 1 && all_waves <= 512;
     const int q_blocks = static_cast<int>((n_tokens + 32 * waves - 1) / (32 * waves));
-    MVX_REQUIRE(n_seqs <= (1 << 23) / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
+    // 2^31 threads in one launch
+    MVX_REQUIRE(n_seqs <= (1 << 25) / waves / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
                 name);
     const unsigned blocks = static_cast<unsigned>(n_seqs * heads * q_blocks);
     return with_element(dtype, name, [&](auto zero) -> int {

@@ -1064,3 +1064,14 @@ def test_window_attention_gradients_of_many_sinks(dtype, case):
                                             grad=f64(up)[one])
         for name, a, c, e in zip(("dq", "dk", "dv"), got, grads, bounds):
             within(a[one], c, e, "%s of sequence %d" % (name, s))
+
+
+def test_a_short_window_takes_the_batch_that_a_long_one_takes():
+    b, n, heads, dim, dtype = (1 << 18) + 40, 33, 16, 8, torch.float16
+    torch.manual_seed(76)
+    q, k, v = (torch.randn(b, n, h, dim, device=DEV, dtype=dtype) for h in (heads, 1, 1))
+    for window in ((200, 0), (2, 1)):
+        out = temporal.window_attention(q, k, v, window)
+        for s in (0, b // 2, b - 1):
+            one = slice(s, s + 1)
+            within(out[one], *orc.attention(f64(q[one]), f64(k[one]), f64(v[one]), window, 0, dtype), "sequence %d" % s)
