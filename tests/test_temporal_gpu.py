@@ -1075,3 +1075,29 @@ def test_a_short_window_takes_the_batch_that_a_long_one_takes():
         for s in (0, b // 2, b - 1):
             one = slice(s, s + 1)
             within(out[one], *orc.attention(f64(q[one]), f64(k[one]), f64(v[one]), window, 0, dtype), "sequence %d" % s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width", [(9001, 257), (5003, 1024), (4500, 100), (9001, 64), (3000, 2000), (1100, 3000), (700, 8193), (600, 16380),
+                                        (1000, 3), (300, 16385)])
+def test_layer_norm_of_more_rows_than_run_at_once(dtype, rows, width):
+    test_layer_norm(dtype, rows, width)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [
+    (1, 1201, 4, 2, 64, (8, 12, 12), True, False, torch.int32, True),
+    (3, 1999, 1, 1, 40, (5, 6), True, True, torch.int64, False),
+    (2, 3001, 2, 0, 36, (5, 4), True, False, torch.float32, True),
+    (5, 701, 3, 1, 24, (12,), False, False, torch.int32, True),
+], ids=str)
+def test_rotate_positions_several_tokens_per_workgroup(dtype, case):
+    if case[3]:
+        test_rotate_positions(dtype, case)
+        return
+    b, n, h, _, d, sections, pairs, shared, ptype, _ = case
+    g = gen(n)
+    q, pos = normal(g, (b, n, h, d), dtype), torch.rand((b, n, len(sections)), generator=g) * 500
+    out, none = temporal.rotate_positions(q, None, pos.to(DEV), sections, pairs=pairs, shared_spectrum=shared)
+    assert none is None
+    within(out, *orc.rotate(f64(q), pos, sections, 10000.0, shared, pairs, dtype), "q alone")
