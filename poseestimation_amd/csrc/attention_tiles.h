@@ -431,7 +431,8 @@ __device__ __forceinline__ bool sees_all(const AttentionShape& s, int w0, int k0
 // key) whose sums end up not finite is therefore computed again, over the pairs it sees alone, with the functions below: if it
 // does see such a value it then holds what the formula gives, otherwise the ordinary result, to rounding.  Columns whose sums
 // are finite met no such value and stay as they are.
-// This walk reads rows lane by lane and is slow.
+// This walk reads rows lane by lane and is slow: one infinite upstream gradient makes the backward of 4 x 4096 x 8 x 64, 255 keys
+// and 4 sinks, take 59 ms instead of 0.11 (each sink's lane walks all queries), one NaN among the values the forward 8 ms.
 
 // Whether the lane's sums are all finite.
 template <int N>

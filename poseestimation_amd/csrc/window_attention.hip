@@ -17,10 +17,10 @@
 // Bound by the matrix and vector units taking turns: the softmax of a block takes about as long as its products, and two waves
 // per SIMD, all that the registers hold, do not hide one behind the other (counters of 8192 tokens x 16 heads of 128, 1040 keys:
 // matrix units busy 31 % of the time, vector units 39 %).  bfloat16, each with the flops of the pairs that are seen: that prompt
-// 97 us (670 Tflop/s), all keys of 2 x 4096 x 16: heads of 64 225 us (610), of 128 330 us (830); 4 x 4096 x 8 x 64 with 256 keys
-// and 4 sinks 36 us (240; blocks cut by the window's edges and the sinks' add a third to the products, and a workgroup's eight
-// tiles leave its first loads exposed).  A large product reaches 1100.  float32 in its three parts: 4 x 4096 x 8 x 64, 1024 keys,
-// 206 us.
+// 98 to 115 us with the clocks (670 to 570 Tflop/s), all keys of 2 x 4096 x 16: heads of 64 228 us (605), of 128 332 us (830);
+// 4 x 4096 x 8 x 64 with 256 keys and 4 sinks 36 us (240; blocks cut by the window's edges and the sinks' add a third to the
+// products, and a workgroup's eight tiles leave its first loads exposed).  A large product reaches 1100.  float32 in its three
+// parts: 4 x 4096 x 8 x 64, 1024 keys, 206 us.
 #include "attention_tiles.h"
 
 namespace mvx {
@@ -296,8 +296,8 @@ extern "C" int mvx_window_attention(const void* q, const int64_t* q_strides, con
     const bool split = dtype == MVX_F32 && waves == 1 && all_waves <= 512;
     const int q_blocks = static_cast<int>((n_tokens + 32 * waves - 1) / (32 * waves));
     // 2^31 threads in one launch
-    MVX_REQUIRE(n_seqs <= (1 << 25) / waves / q_blocks / heads, MVX_ERR_UNSUPPORTED, "%s: too many sequences, heads and tokens for one launch",
-                name);
+    MVX_REQUIRE(n_seqs <= (1 << 25) / waves / q_blocks / heads, MVX_ERR_UNSUPPORTED,
+                "%s: too many sequences, heads and tokens for one launch", name);
     const unsigned blocks = static_cast<unsigned>(n_seqs * heads * q_blocks);
     return with_element(dtype, name, [&](auto zero) -> int {
         using T = decltype(zero);

@@ -9,7 +9,8 @@
 //   2. keys in lanes, walking the tiles of queries that see them, over all heads that share the keys: dk and dv.
 // In the second a block of sink keys is seen by the whole rest of the sequence.  The queries behind the block's own window
 // are therefore cut into chunks that a third kernel takes, between the two: a workgroup per chunk and 32 sinks, its waves
-// on queries of their own, its sum left in float32.  A fourth adds the chunks in order, and the block of keys starts from that.
+// on queries of their own, its sum left in float32.  A fourth adds the chunks in order, and the block of keys adds that to its own
+// (but for many sinks, whose blocks fill the GPU and walk all queries).
 // delta is taken from the output together with what its rounding left: a row that one key dominates has dp - delta near zero
 // there, and the output rounded to bfloat16 alone would be off by as much as the difference (three keys of unit spread: dq and dk
 // off by 0.0033 of their size instead of 0.0025, of twice that spread 0.0066 instead of 0.0024).

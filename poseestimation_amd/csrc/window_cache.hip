@@ -5,7 +5,8 @@
 // sinks + (t - sinks) % window, so the slots hold exactly what token t sees with left = window - 1, right = 0: the first
 // tokens and the last `window` ones.  The order of the slots does not matter to a softmax, so nothing is ever moved.
 //
-// One step reads every held key and value once and is bound by that.  Three kernels share the work:
+// One step is bound by reading the held keys and values: once for up to 32 heads that share them with 16-bit types, for four with
+// float32, for two in a short ring (the caches may hold them from then on).  Three kernels share the work:
 //   window_step_tiles   16-bit types: a wave takes 32 slots at a time through tiles of its own and multiplies them with all
 //                       heads that share them on the matrix units (up to 32 heads cost what one costs)
 //   window_step_lanes   float32, and short rings of any type: 4, 8 or 16 lanes hold one key (8 values per lane), so a wave
@@ -13,8 +14,9 @@
 //   window_step_join    the slots of a long ring are cut into shares, a workgroup each, which leave their sums in float32; this
 //                       adds them and advances the lengths (all readers of the old length are done by then)
 // A short ring is one workgroup's work for all heads of its stream: window_step_lanes then finishes the step in one launch.
-// 64 streams x 4112 slots x 4 heads of 128 bfloat16, 16 heads reading them: 103 us (5.2 TB/s) and 5 us for the join; one stream x
-// 68 slots x 8 heads of 64 float32: 6.8 us.  The filling copies; 32 x 4112 slots x 4 heads of 128 bfloat16: 97 us (5.5 TB/s).
+// 64 streams x 4112 slots x 4 heads of 128 bfloat16, 16 heads reading them: 99 us (5.4 TB/s) and 5 us for the join; 32 x 4112 x 4 x
+// 128 float32, 8 heads: 101 us together (5.3 TB/s), 32 heads 160 us; one stream x 68 slots x 8 heads of 64 float32: 6.9 us.  The
+// filling copies; 32 x 4112 slots x 4 heads of 128 bfloat16: 97 us (5.5 TB/s).
 #include "attention_tiles.h"
 
 namespace mvx {
